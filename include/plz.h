@@ -605,6 +605,75 @@ int32_t plz_advance(int32_t* pos, int32_t n, void* stream);
 int32_t plz_sample(const float* logits, int64_t ld, int32_t rows, int32_t V, float temperature, int32_t top_k, uint32_t seed, const int32_t* pos,
                    int64_t* out, void* stream);
 
+/* ---- A batch of requests of different lengths: paged keys and values, logits with a request's settings ----------------------------------
+ * (No counterpart in the reference.) The cache is a pool of pages of page_size token rows; a request's row of `table` names its pages in order, and
+ * position t of the request is row t % page_size of page table[t / page_size]. All counts live in device memory, so a captured step can be replayed.
+ *
+ * plz_page_plan: pages and slots for the next step. Request b has cached[b] tokens in ceil(cached[b] / page_size) pages and brings new_tokens[b] >= 0 tokens;
+ *   a negative number ends it: its pages go back, its length becomes 0. Free pages are free_pages[0 .. *n_free), taken from the end by the requests in order;
+ *   what ended requests give back is on top afterwards, in their order, and serves the next step.
+ *   status[b] (int32 [B]): 0 done; 1 the free pages do not suffice for it (nor for any later request that needs one); 2 it does not fit: cached[b] < 0, more tokens than `width`
+ *   pages or 2^31 - 1 hold, rows past max_rows or more than row_pitch. A request with status 1 or 2 keeps its pages and its length.
+ *   starts (int32 [B + 1]): first row of each request among the step's token rows: the running sum of the new tokens, or b * row_pitch where row_pitch > 0.
+ *   slots, positions (int32 [max_rows]): page * page_size + row in the page, and position, of every token row; -1 for rows of nobody or of a request with status 1 or 2.
+ *   lengths (int32 [B]), n_free_out: afterwards; may be `cached` and `n_free` themselves, nothing else may overlap. table gets the new pages.
+ *   B <= 16384, B * width < 2^30, n_pages * page_size < 2^31. A page outside the pool gives slot -1.
+ * plz_page_write: row slots[i] of the pools = row i of k and v (row_bytes of any type), i < rows; a slot outside the pool (-1) is skipped. Slots other than those must
+ *   differ: of two rows for one slot parts of both may remain. Strides in BYTES; bases, strides and row_bytes multiples of 16.
+ * plz_attn_decode_paged: attention of one new token per request (its key and value stored already): out[b, h] = softmax(q[b, h] . K[0 .. lengths[b]) * scale) V[0 .. lengths[b])
+ *   over the request's pages, key / value head h / (Hq / Hkv). bf16, q and out [B, Hq * head_dim], pools [n_pages, page_size, Hkv * head_dim] with the element strides
+ *   between pages and between rows, head_dim 64, 128 or 256. lengths[b] <= 0 gives zeros. Nothing behind a request's length is read into the result. A page outside the pool
+ *   is left out of the softmax and a length past `width` pages is cut, either of them (and a negative length) stores 1 to *bad (device int32, may be NULL); values are finite.
+ *   ws: plz_attn_decode_paged_ws_bytes, 16-byte aligned, for any B and lengths; calls that may run at the same time need one each. Bits repeat from run to run; a request's may change with the other requests'
+ *   lengths, which move the places where its sums are cut.
+ * plz_adjust_logits: out = logits [rows, V] (dtype 0 bf16, 1 fp32, computed in fp32, out may be logits) after, in this order,
+ *   repetition r: x > 0 ? x / r : x * r for every token among tokens[0 .. lengths[row]) (int64 [rows, >= lengths], rows ldk apart);
+ *   frequency f, presence p: x - f * c - p for tokens that occur c > 0 times among tokens[prompt_lengths[row] .. lengths[row]);
+ *   bias: x + the biases of the token, fp32 bias[row, i] for token bias_ids[row, i], in the order of i;
+ *   mask: -inf where bit t % 32 of word t / 32 of the row's mask (int32, rows ldm apart) is 0.
+ *   repetition, presence, frequency: fp32 [rows], or NULL: the value of the field behind it for all rows. prompt_lengths NULL: 0. lengths NULL: no tokens; negative ones count as 0
+ *   and ones past max_tokens (the columns of `tokens`, < 2^30) as max_tokens. Ids outside [0, V) are nobody's. bias_ids and bias: n_bias <= 4096 columns, rows ldb apart. mask NULL: all allowed. */
+typedef struct plz_page_plan {
+    const int32_t* cached; const int32_t* new_tokens;
+    int32_t* table; int64_t ldt;
+    int32_t* free_pages; const int32_t* n_free;
+    int32_t* lengths; int32_t* n_free_out;
+    int32_t* starts; int32_t* slots; int32_t* positions; int32_t* status;
+    int32_t B, width, page_size, n_pages, max_rows, row_pitch;
+} plz_page_plan_t;
+int32_t plz_page_plan(const plz_page_plan_t* args, void* stream);
+typedef struct plz_page_write {
+    const void* k; const void* v; int64_t ldk, ldv;
+    void* k_pages; void* v_pages; int64_t page_stride, tok_stride;
+    const int32_t* slots;
+    int32_t rows, row_bytes, page_size, n_pages;
+} plz_page_write_t;
+int32_t plz_page_write(const plz_page_write_t* args, void* stream);
+typedef struct plz_attn_decode_paged {
+    const void* q; int64_t ldq;
+    const void* k_pages; const void* v_pages; int64_t page_stride, tok_stride;
+    const int32_t* table; int64_t ldt;
+    const int32_t* lengths;
+    void* out; int64_t ldo;
+    int32_t* bad;
+    int32_t B, width, page_size, n_pages, Hq, Hkv, head_dim;
+    float scale;
+} plz_attn_decode_paged_t;
+int64_t plz_attn_decode_paged_ws_bytes(int32_t Hq, int32_t Hkv, int32_t head_dim);
+int32_t plz_attn_decode_paged(const plz_attn_decode_paged_t* args, void* ws, int64_t ws_bytes, void* stream);
+typedef struct plz_adjust_logits {
+    const void* logits; int64_t ld;
+    void* out; int64_t ldo;
+    const int64_t* tokens; int64_t ldk;
+    const int32_t* lengths; const int32_t* prompt_lengths;
+    const float* repetition; const float* presence; const float* frequency;
+    const int64_t* bias_ids; const float* bias; int64_t ldb;
+    const int32_t* mask; int64_t ldm;
+    float repetition_all, presence_all, frequency_all;
+    int32_t rows, V, max_tokens, n_bias;
+} plz_adjust_logits_t;
+int32_t plz_adjust_logits(int32_t dtype, const plz_adjust_logits_t* args, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

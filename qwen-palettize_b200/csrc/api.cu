@@ -1209,6 +1209,82 @@ int32_t plz_sample(const float* logits, int64_t ld, int32_t rows, int32_t V, flo
     return launch_sample(logits, ld, rows, V, temperature, top_k, seed, pos, (long long*)out, (cudaStream_t)stream);
 }
 
+// ---- a batch of requests of different lengths -----------------------------------------------------------------
+int32_t plz_page_plan(const plz_page_plan_t* a, void* stream) {
+    if (!a || !a->n_free || !a->n_free_out || !a->starts || (a->B > 0 && (!a->cached || !a->new_tokens || !a->lengths || !a->status || (a->width > 0 && !a->table))) ||
+        (a->n_pages > 0 && !a->free_pages) || (a->max_rows > 0 && (!a->slots || !a->positions))) { set_last_error("null pointer"); return PLZ_ERR_NULL; }
+    if (a->B < 0 || a->width < 0 || a->page_size <= 0 || a->n_pages < 0 || a->max_rows < 0 || a->row_pitch < 0 || (a->B > 1 && a->ldt < a->width)) {
+        set_last_error("page_plan: bad shape B=%d width=%d page=%d pages=%d rows=%d pitch=%d", a->B, a->width, a->page_size, a->n_pages, a->max_rows, a->row_pitch); return PLZ_ERR_BAD_SHAPE;
+    }
+    if (a->B > 16384 || (int64_t)a->B * a->width >= (1 << 30) || (int64_t)a->n_pages * a->page_size > 0x7FFFFFFF || a->max_rows > (1 << 30)) {
+        set_last_error("page_plan: more than 16384 requests, 2^30 table entries or rows, or 2^31 slots"); return PLZ_ERR_TOO_LARGE;
+    }
+    return launch_page_plan(*a, (cudaStream_t)stream);
+}
+
+int32_t plz_page_write(const plz_page_write_t* a, void* stream) {
+    if (!a) { set_last_error("null pointer"); return PLZ_ERR_NULL; }
+    if (a->rows < 0 || a->row_bytes <= 0 || a->page_size <= 0 || a->n_pages < 0 || a->ldk < 0 || a->ldv < 0 || a->tok_stride < a->row_bytes || a->page_stride < a->row_bytes) {
+        set_last_error("page_write: bad shape rows=%d bytes=%d page=%d pages=%d", a->rows, a->row_bytes, a->page_size, a->n_pages); return PLZ_ERR_BAD_SHAPE;
+    }
+    if ((int64_t)a->n_pages * a->page_size > 0x7FFFFFFF || a->rows > (1 << 30)) { set_last_error("page_write: more than 2^31 slots or 2^30 rows"); return PLZ_ERR_TOO_LARGE; }
+    if (a->rows == 0 || a->n_pages == 0) return PLZ_OK;
+    if (!a->k || !a->v || !a->k_pages || !a->v_pages || !a->slots) { set_last_error("null pointer"); return PLZ_ERR_NULL; }
+    if ((((uintptr_t)a->k | (uintptr_t)a->v | (uintptr_t)a->k_pages | (uintptr_t)a->v_pages) & 15) || ((a->ldk | a->ldv | a->tok_stride | a->page_stride | a->row_bytes) & 15)) {
+        set_last_error("page_write: rows must be whole 16-byte units"); return PLZ_ERR_BAD_ALIGN;
+    }
+    return launch_page_write(*a, (cudaStream_t)stream);
+}
+
+int64_t plz_attn_decode_paged_ws_bytes(int32_t Hq, int32_t Hkv, int32_t head_dim) {
+    if (Hq <= 0 || Hkv <= 0 || head_dim <= 0) return 0;
+    return paged_attn_ws_bytes(Hq, Hkv, head_dim);
+}
+
+int32_t plz_attn_decode_paged(const plz_attn_decode_paged_t* a, void* ws, int64_t ws_bytes, void* stream) {
+    if (!a) { set_last_error("null pointer"); return PLZ_ERR_NULL; }
+    if (a->B < 0 || a->width < 0 || a->page_size <= 0 || a->n_pages < 0 || a->Hq <= 0 || a->Hkv <= 0 || a->Hq % a->Hkv || (a->head_dim != 64 && a->head_dim != 128 && a->head_dim != 256)) {
+        set_last_error("attn_decode_paged: needs head_dim 64, 128 or 256 and Hq a multiple of Hkv (B=%d width=%d page=%d pages=%d Hq=%d Hkv=%d d=%d)", a->B, a->width, a->page_size, a->n_pages,
+                       a->Hq, a->Hkv, a->head_dim);
+        return PLZ_ERR_BAD_SHAPE;
+    }
+    const int64_t qd = (int64_t)a->Hq * a->head_dim, kd = (int64_t)a->Hkv * a->head_dim;
+    if (qd > (1 << 24) || (a->B > 1 && (a->ldq < qd || a->ldo < qd || a->ldt < a->width)) || a->tok_stride < kd || a->page_stride < kd) {
+        set_last_error("attn_decode_paged: rows overlap (%lld query, %lld key columns)", (long long)qd, (long long)kd); return PLZ_ERR_BAD_SHAPE;
+    }
+    if (a->B == 0) return PLZ_OK;
+    if (!a->q || !a->out || !a->lengths || (a->width > 0 && !a->table) || (a->n_pages > 0 && (!a->k_pages || !a->v_pages))) { set_last_error("null pointer"); return PLZ_ERR_NULL; }
+    if ((((uintptr_t)a->q | (uintptr_t)a->out | (uintptr_t)a->k_pages | (uintptr_t)a->v_pages | (uintptr_t)ws) & 15) || ((a->ldq | a->ldo | a->page_stride | a->tok_stride) & 7)) {
+        set_last_error("attn_decode_paged: rows must be 16-byte aligned"); return PLZ_ERR_BAD_ALIGN;
+    }
+    // the kernel counts in 16-byte units, 32 bits of them
+    const uint64_t page16 = (uint64_t)a->page_stride / 8, tok16 = (uint64_t)a->tok_stride / 8;
+    if (page16 > 0xFFFFFFFFull || tok16 > 0xFFFFFFFFull || (a->n_pages > 0 && (uint64_t)(a->n_pages - 1) * page16 + (uint64_t)(a->page_size - 1) * tok16 > 0xFFFFFFFFull)) {
+        set_last_error("attn_decode_paged: a pool of more than 64 GiB"); return PLZ_ERR_TOO_LARGE;
+    }
+    if (a->q == a->out) { set_last_error("attn_decode_paged: out may not be q"); return PLZ_ERR_UNSUPPORTED; }
+    return launch_paged_attn(*a, ws, ws ? ws_bytes : 0, (cudaStream_t)stream);
+}
+
+int32_t plz_adjust_logits(int32_t dtype, const plz_adjust_logits_t* a, void* stream) {
+    int rc = check_dtype(dtype);
+    if (rc) return rc;
+    if (!a) { set_last_error("null pointer"); return PLZ_ERR_NULL; }
+    const int64_t words = ((int64_t)a->V + 31) / 32;
+    if (a->rows < 0 || a->V <= 0 || a->max_tokens < 0 || a->n_bias < 0 || a->ldk < 0 || a->ldb < 0 || a->ldm < 0 || (a->rows > 1 && (a->ld < a->V || a->ldo < a->V)) ||
+        (a->ldk && a->rows > 1 && a->ldk < a->max_tokens) || (a->ldb && a->rows > 1 && a->ldb < a->n_bias) || (a->ldm && a->rows > 1 && a->ldm < words)) {
+        set_last_error("adjust_logits: bad shape rows=%d V=%d tokens=%d biases=%d", a->rows, a->V, a->max_tokens, a->n_bias); return PLZ_ERR_BAD_SHAPE;
+    }
+    if (a->rows > 65535 || a->max_tokens >= (1 << 30) || a->n_bias > 4096 || a->V > (1 << 30)) {
+        set_last_error("adjust_logits: more than 65535 rows, 4096 biases a row, or 2^30 tokens"); return PLZ_ERR_TOO_LARGE;
+    }
+    if (a->rows == 0) return PLZ_OK;
+    if (!a->logits || !a->out || (a->lengths && a->max_tokens > 0 && !a->tokens) || (a->n_bias > 0 && (!a->bias_ids || !a->bias))) { set_last_error("null pointer"); return PLZ_ERR_NULL; }
+    const uintptr_t size = dtype == 1 ? 4 : 2;
+    if (((uintptr_t)a->logits | (uintptr_t)a->out) & (size - 1)) { set_last_error("adjust_logits: misaligned logits"); return PLZ_ERR_BAD_ALIGN; }
+    return launch_adjust_logits(dtype, *a, (cudaStream_t)stream);
+}
+
 // ---- one decode step of a palettized model -----------------------------------------------------------------
 // Forty-odd launches per step of four layers: from Python each costs 15 to 20 us of host time, more than the kernels take.
 // One sequence, four layers: 830 -> 265 us a step; 64 sequences 838 -> 650 us (with gate / up and q / k / v in one launch each).

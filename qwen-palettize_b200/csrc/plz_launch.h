@@ -250,6 +250,22 @@ int launch_put_words(long long* dst, const long long* values, int n, cudaStream_
 int launch_sample(const float* logits, long long ld, int rows, int V, float temperature, int top_k, uint32_t seed, const int* pos, long long* out,
                   cudaStream_t stream);
 
+// paged.cu, paged_attention.cu, adjust_logits.cu: a batch of requests of different lengths
+inline int sms_of_current_device() {
+    int dev = 0, n = 0;
+    cudaGetDevice(&dev);
+    return cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) == cudaSuccess && n > 0 ? n : 1;
+}
+using PagePlanArgs = plz_page_plan_t;
+int launch_page_plan(const PagePlanArgs& a, cudaStream_t stream);
+using PageWriteArgs = plz_page_write_t;
+int launch_page_write(const PageWriteArgs& a, cudaStream_t stream);
+using PagedAttnArgs = plz_attn_decode_paged_t;
+long long paged_attn_ws_bytes(int Hq, int Hkv, int head_dim);
+int launch_paged_attn(const PagedAttnArgs& a, void* ws, long long ws_bytes, cudaStream_t stream);
+using AdjustLogitsArgs = plz_adjust_logits_t;
+int launch_adjust_logits(int dtype, const AdjustLogitsArgs& a, cudaStream_t stream);
+
 // ---- train_ops.cu ------------------------------------------------------------------------------
 struct AdamParams {
     float* master; float* m; float* v;

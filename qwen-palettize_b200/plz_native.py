@@ -114,6 +114,30 @@ class LatentAttn(C.Structure):
                 ("B", C.c_int32), ("n", C.c_int32), ("H", C.c_int32), ("R", C.c_int32), ("dr", C.c_int32), ("scale", C.c_float)]
 
 
+class PagePlan(C.Structure):
+    _fields_ = [("cached", C.c_void_p), ("new_tokens", C.c_void_p), ("table", C.c_void_p), ("ldt", C.c_int64), ("free_pages", C.c_void_p), ("n_free", C.c_void_p),
+                ("lengths", C.c_void_p), ("n_free_out", C.c_void_p), ("starts", C.c_void_p), ("slots", C.c_void_p), ("positions", C.c_void_p), ("status", C.c_void_p),
+                ("B", C.c_int32), ("width", C.c_int32), ("page_size", C.c_int32), ("n_pages", C.c_int32), ("max_rows", C.c_int32), ("row_pitch", C.c_int32)]
+
+
+class PageWrite(C.Structure):
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("ldk", C.c_int64), ("ldv", C.c_int64), ("k_pages", C.c_void_p), ("v_pages", C.c_void_p), ("page_stride", C.c_int64),
+                ("tok_stride", C.c_int64), ("slots", C.c_void_p), ("rows", C.c_int32), ("row_bytes", C.c_int32), ("page_size", C.c_int32), ("n_pages", C.c_int32)]
+
+
+class AttnDecodePaged(C.Structure):
+    _fields_ = [("q", C.c_void_p), ("ldq", C.c_int64), ("k_pages", C.c_void_p), ("v_pages", C.c_void_p), ("page_stride", C.c_int64), ("tok_stride", C.c_int64), ("table", C.c_void_p),
+                ("ldt", C.c_int64), ("lengths", C.c_void_p), ("out", C.c_void_p), ("ldo", C.c_int64), ("bad", C.c_void_p), ("B", C.c_int32), ("width", C.c_int32),
+                ("page_size", C.c_int32), ("n_pages", C.c_int32), ("Hq", C.c_int32), ("Hkv", C.c_int32), ("head_dim", C.c_int32), ("scale", C.c_float)]
+
+
+class AdjustLogits(C.Structure):
+    _fields_ = [("logits", C.c_void_p), ("ld", C.c_int64), ("out", C.c_void_p), ("ldo", C.c_int64), ("tokens", C.c_void_p), ("ldk", C.c_int64), ("lengths", C.c_void_p),
+                ("prompt_lengths", C.c_void_p), ("repetition", C.c_void_p), ("presence", C.c_void_p), ("frequency", C.c_void_p), ("bias_ids", C.c_void_p), ("bias", C.c_void_p),
+                ("ldb", C.c_int64), ("mask", C.c_void_p), ("ldm", C.c_int64), ("repetition_all", C.c_float), ("presence_all", C.c_float), ("frequency_all", C.c_float),
+                ("rows", C.c_int32), ("V", C.c_int32), ("max_tokens", C.c_int32), ("n_bias", C.c_int32)]
+
+
 _I32, _I64, _P, _F = C.c_int32, C.c_int64, C.c_void_p, C.c_float
 _WP, _LP, _GP, _NP = C.POINTER(Weight), C.POINTER(Lora), C.POINTER(Logits), C.POINTER(Noise)
 
@@ -200,13 +224,18 @@ SIGNATURES = {
     "plz_attn_prep": [_I32, C.POINTER(AttnPrep), _P],
     "plz_attn_bias_ws_bytes": [_I32, _I32, _I32, _I32, _I32],
     "plz_attn_bias": [_I32, C.POINTER(AttnBias), _P, _I64, _P],
+    "plz_page_plan": [C.POINTER(PagePlan), _P],
+    "plz_page_write": [C.POINTER(PageWrite), _P],
+    "plz_attn_decode_paged_ws_bytes": [_I32, _I32, _I32],
+    "plz_attn_decode_paged": [C.POINTER(AttnDecodePaged), _P, _I64, _P],
+    "plz_adjust_logits": [_I32, C.POINTER(AdjustLogits), _P],
     "plz_advance": [_P, _I32, _P],
     "plz_put_words": [_P, _P, _I32, _P],
     "plz_sample": [_P, _I64, _I32, _I32, _F, _I32, C.c_uint32, _P, _P, _P],
     "plz_distill_loss": [_P, _I64, _P, _I64, _I32, _I32, _F, _F, _F, _P, _P, _P, _I64, _I32, _P],
 }
 _RESTYPES = {"plz_last_error": C.c_char_p, "plz_launch_count": C.c_uint64, "plz_attn_decode_ws_bytes": C.c_int64, "plz_decode_ws_bytes": C.c_int64,
-             "plz_attn_bias_ws_bytes": C.c_int64, "plz_chunk_ws_bytes": C.c_int64, "plz_latent_attn_ws_bytes": C.c_int64}
+             "plz_attn_decode_paged_ws_bytes": C.c_int64, "plz_attn_bias_ws_bytes": C.c_int64, "plz_chunk_ws_bytes": C.c_int64, "plz_latent_attn_ws_bytes": C.c_int64}
 
 
 def lib():
@@ -264,6 +293,16 @@ def _need_cuda(*ts):
     for t in ts:
         if t is not None and not t.is_cuda:
             raise PlzError("libplz works on CUDA tensors only (no CPU path exists)")
+
+
+def need_here(*ts):
+    """All tensors (None aside) on the current device."""
+    here = torch._C._cuda_getDevice() if torch.cuda.is_initialized() else torch.cuda.current_device() if torch.cuda.is_available() else -1
+    for t in ts:
+        if t is not None and not t.is_cuda:
+            raise PlzError("libplz works on CUDA tensors only (no CPU path exists)")
+        if t is not None and t.device.index != here:
+            raise PlzError(f"a tensor on {t.device}, but the current device is cuda:{here}")
 
 
 def weight_desc(packed: torch.Tensor, palette: torch.Tensor, N: int, K: int, gs_n: int, gs_k: int) -> Weight:

@@ -629,6 +629,86 @@ def attention_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
     return out
 
 
+@dataclass
+class PagePlan:
+    """What plan_pages says about a step, int32 on the device."""
+    lengths: torch.Tensor     # [B] tokens of each request, the new ones among them
+    n_free: torch.Tensor      # [1] free pages left
+    starts: torch.Tensor      # [B + 1] first token row of each request
+    slots: torch.Tensor       # [max_rows] page * page_size + row in the page, -1: none
+    positions: torch.Tensor   # [max_rows] position in its request, -1: none
+    status: torch.Tensor      # [B] 0 done, 1 out of pages, 2 does not fit
+
+
+def _int32(t: torch.Tensor, shape, what: str):
+    assert t.dtype == torch.int32 and tuple(t.shape) == tuple(shape) and t.is_contiguous(), f"{what}: contiguous int32 {tuple(shape)}"
+    return t
+
+
+def plan_pages(lengths: torch.Tensor, new_tokens: torch.Tensor, table: torch.Tensor, free_pages: torch.Tensor, n_free: torch.Tensor, page_size: int, max_rows: int,
+               row_pitch: int = 0, lengths_out: torch.Tensor | None = None, n_free_out: torch.Tensor | None = None) -> PagePlan:
+    """Pages and slots of the next step of a batch of requests, without a look at the device's numbers from the host. lengths, new_tokens int32 [B]: cached tokens and tokens that
+    the step brings, in order of the requests (row_pitch > 0: row_pitch rows for every request); a negative number ends the request and gives its pages back. table int32 [B, width] names
+    the requests' pages and gets the new ones; free_pages int32 [n_pages], whose first n_free (int32 [1]) entries are free, taken from the end. A request that the free pages or `width` pages do not
+    suffice for keeps what it has (status). lengths_out, n_free_out: where the new counts go, `lengths` and `n_free` themselves for a step that is captured; None: new tensors."""
+    B = lengths.shape[0]
+    _int32(lengths, (B,), "lengths"), _int32(new_tokens, (B,), "new_tokens"), _int32(n_free, (1,), "n_free"), _int32(free_pages, free_pages.shape[:1], "free_pages")
+    assert table.dtype == torch.int32 and table.dim() == 2 and table.shape[0] == B and table.stride(1) == 1, "table: int32 [B, width] with unit column stride"
+    for t, n in ((lengths_out, B), (n_free_out, 1)):
+        assert t is None or _int32(t, (n,), "lengths_out, n_free_out") is t
+    P.need_here(lengths, new_tokens, table, free_pages, n_free, lengths_out, n_free_out)
+    new = lambda n: torch.empty(n, dtype=torch.int32, device=lengths.device)
+    p = PagePlan(lengths_out if lengths_out is not None else new(B), n_free_out if n_free_out is not None else new(1), new(B + 1), new(max_rows), new(max_rows), new(B))
+    a = P.PagePlan(lengths.data_ptr(), new_tokens.data_ptr(), table.data_ptr(), table.stride(0), free_pages.data_ptr(), n_free.data_ptr(), p.lengths.data_ptr(), p.n_free.data_ptr(),
+                   p.starts.data_ptr(), p.slots.data_ptr(), p.positions.data_ptr(), p.status.data_ptr(), B, table.shape[1], page_size, free_pages.shape[0], max_rows, row_pitch)
+    P.check(P.lib().plz_page_plan(C.byref(a), P.stream_ptr()), "plz_page_plan")
+    return p
+
+
+def _pools(k_pages: torch.Tensor, v_pages: torch.Tensor, cols: int):
+    assert k_pages.dim() == 3 and k_pages.shape == v_pages.shape and k_pages.stride() == v_pages.stride() and k_pages.dtype == v_pages.dtype, "pools of one shape, layout and type"
+    assert k_pages.shape[2] == cols and k_pages.stride(2) == 1, f"pools: [n_pages, page_size, {cols}] with unit column stride"
+
+
+def write_pages(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor):
+    """Rows of k and v [rows, width] into their slots of the pools [n_pages, page_size, width], any type of one size; rows with slot -1 are skipped, the others' slots differ."""
+    assert k.dim() == 2 and k.shape == v.shape and k.dtype == v.dtype == k_pages.dtype and k.stride(1) == v.stride(1) == 1, "k, v: rows of the pools' type, unit column stride"
+    rows, W = k.shape
+    _pools(k_pages, v_pages, W)
+    _int32(slots, (rows,), "slots")
+    P.need_here(k, v, slots, k_pages, v_pages)
+    n = k.element_size()
+    a = P.PageWrite(k.data_ptr(), v.data_ptr(), k.stride(0) * n, v.stride(0) * n, k_pages.data_ptr(), v_pages.data_ptr(), k_pages.stride(0) * n, k_pages.stride(1) * n, slots.data_ptr(),
+                    rows, W * n, k_pages.shape[1], k_pages.shape[0])
+    P.check(P.lib().plz_page_write(C.byref(a), P.stream_ptr()), "plz_page_write")
+
+
+def attention_decode_paged(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tensor, lengths: torch.Tensor, n_heads: int, n_kv_heads: int,
+                           head_dim: int = 128, scale: float | None = None, out: torch.Tensor | None = None, bad: torch.Tensor | None = None) -> torch.Tensor:
+    """Attention of one new token per request over the request's own length of cached tokens (its own among them). q bf16 [B, n_heads * head_dim], pools bf16
+    [n_pages, page_size, n_kv_heads * head_dim], table int32 [B, width], lengths int32 [B] on the device (0: zeros). Returns bf16 [B, n_heads * head_dim]. bad (int32 [1]) is set to 1
+    where a page lies outside the pool (its tokens are left out) or a length outside the table."""
+    _mat(q, n_heads * head_dim)
+    B = q.shape[0]
+    _pools(k_pages, v_pages, n_kv_heads * head_dim)
+    assert k_pages.dtype == torch.bfloat16, "pools: bf16"
+    assert table.dtype == torch.int32 and table.dim() == 2 and table.shape[0] == B and table.stride(1) == 1, "table: int32 [B, width] with unit column stride"
+    _int32(lengths, (B,), "lengths")
+    if bad is not None:
+        _int32(bad, (1,), "bad")
+    if out is None:
+        out = torch.empty(B, n_heads * head_dim, dtype=torch.bfloat16, device=q.device)
+    assert _mat(out, n_heads * head_dim).shape[0] == B
+    P.need_here(q, k_pages, v_pages, table, lengths, out, bad)
+    nbytes = int(P.lib().plz_attn_decode_paged_ws_bytes(n_heads, n_kv_heads, head_dim))
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
+    a = P.AttnDecodePaged(q.data_ptr(), q.stride(0), k_pages.data_ptr(), v_pages.data_ptr(), k_pages.stride(0), k_pages.stride(1), table.data_ptr(), table.stride(0), lengths.data_ptr(),
+                          out.data_ptr(), out.stride(0), bad.data_ptr() if bad is not None else None, B, table.shape[1], k_pages.shape[1], k_pages.shape[0], n_heads, n_kv_heads, head_dim,
+                          float(scale) if scale is not None else head_dim ** -0.5)
+    P.check(P.lib().plz_attn_decode_paged(C.byref(a), ws.data_ptr(), nbytes, P.stream_ptr()), "plz_attn_decode_paged")
+    return out
+
+
 def decode_hidden(ids: torch.Tensor, embed: torch.Tensor, layers, names, norms, k_cache: torch.Tensor, v_cache: torch.Tensor, T: int, final_norm: torch.Tensor,
                   cos: torch.Tensor, sin: torch.Tensor, n_heads: int, n_kv_heads: int, intermediate: int, eps: float):
     """One token per sequence through all layers of a hard-palettized model, one native call. ids int64 [B]; layers: dicts with the PackedWeight of

@@ -255,6 +255,53 @@ def advance(pos: torch.Tensor, n: int):
     P.check(P.lib().plz_advance(pos.data_ptr(), n, P.stream_ptr()), "plz_advance")
 
 
+def _per_row(v, rows: int, what: str):
+    """(tensor or None, value for all rows) of a setting given as one number or as fp32 [rows]."""
+    if not isinstance(v, torch.Tensor):
+        return None, float(v)
+    assert v.dtype == torch.float32 and tuple(v.shape) == (rows,) and v.is_contiguous(), f"{what}: a number or contiguous fp32 [{rows}]"
+    return v, 0.0
+
+
+def _columns(t: torch.Tensor, rows: int, dtype, what: str):
+    assert t.dtype == dtype and t.dim() == 2 and t.shape[0] == rows and (t.stride(1) == 1 or t.shape[1] <= 1), f"{what}: {dtype} [{rows}, n] with unit column stride"
+    return t
+
+
+def adjust_logits(logits: torch.Tensor, tokens=None, lengths=None, prompt_lengths=None, repetition=1.0, presence=0.0, frequency=0.0, bias_ids=None, bias=None, mask=None,
+                  out: torch.Tensor | None = None) -> torch.Tensor:
+    """Logits [rows, V] (bf16 or fp32) after a request's settings, in this order: x / repetition where x > 0, else x * repetition, for tokens that occur among the row's first lengths[row] of
+    `tokens` (int64 [rows, n], lengths int32 [rows]); x - frequency * count - presence for those that occur `count` times behind the first prompt_lengths[row] of them; the biases
+    (fp32 [rows, n]) of the tokens bias_ids (int64 [rows, n], -1: nobody's); -inf where bit t % 32 of mask[row, t // 32] (int32, [rows or 1, ceil(V / 32)]) is 0. repetition, presence, frequency:
+    a number or fp32 [rows]. out may be `logits`."""
+    assert logits.dim() == 2 and (logits.stride(1) == 1 or logits.shape[1] <= 1), "logits: [rows, V] with unit column stride"
+    rows, V = logits.shape
+    dtype = code(logits.dtype)
+    if out is None:
+        out = torch.empty(rows, V, dtype=logits.dtype, device=logits.device)
+    assert out.shape == logits.shape and out.dtype == logits.dtype and (out.stride(1) == 1 or V <= 1), "out: the shape and type of logits"
+    assert (tokens is None) == (lengths is None) and (prompt_lengths is None or tokens is not None), "tokens and lengths go together"
+    assert (bias_ids is None) == (bias is None), "bias_ids and bias go together"
+    if tokens is not None:
+        _columns(tokens, rows, torch.int64, "tokens")
+        for t, what in ((lengths, "lengths"), (prompt_lengths, "prompt_lengths")):
+            assert t is None or (t.dtype == torch.int32 and tuple(t.shape) == (rows,) and t.is_contiguous()), f"{what}: contiguous int32 [{rows}]"
+    if bias is not None:
+        _columns(bias_ids, rows, torch.int64, "bias_ids"), _columns(bias, rows, torch.float32, "bias")
+        assert bias.shape == bias_ids.shape and bias.stride(0) == bias_ids.stride(0), "bias: the shape and layout of bias_ids"
+    if mask is not None:
+        assert mask.dtype == torch.int32 and mask.dim() == 2 and mask.shape[0] in (1, rows) and mask.shape[1] == (V + 31) // 32 and (mask.stride(1) == 1 or V <= 32), \
+            f"mask: int32 [{rows} or 1, {(V + 31) // 32}] with unit column stride"
+    (r, r_all), (p, p_all), (f, f_all) = (_per_row(v, rows, what) for v, what in ((repetition, "repetition"), (presence, "presence"), (frequency, "frequency")))
+    P.need_here(logits, out, tokens, lengths, prompt_lengths, r, p, f, bias_ids, bias, mask)
+    d = P.AdjustLogits(logits.data_ptr(), logits.stride(0), out.data_ptr(), out.stride(0), _ptr(tokens), tokens.stride(0) if tokens is not None else 0, _ptr(lengths), _ptr(prompt_lengths),
+                       _ptr(r), _ptr(p), _ptr(f), _ptr(bias_ids), _ptr(bias), bias.stride(0) if bias is not None else 0, _ptr(mask),
+                       mask.stride(0) if mask is not None and mask.shape[0] == rows else 0, r_all, p_all, f_all, rows, V, tokens.shape[1] if tokens is not None else 0,
+                       bias.shape[1] if bias is not None else 0)
+    P.check(P.lib().plz_adjust_logits(dtype, C.byref(d), P.stream_ptr()), "plz_adjust_logits")
+    return out
+
+
 def sample(logits: torch.Tensor, pos: torch.Tensor, temperature: float = 0.0, top_k: int = 0, seed: int = 0) -> torch.Tensor:
     """Next token int64 [rows] of fp32 logits [rows, V]; temperature 0 is greedy."""
     assert logits.dtype == torch.float32 and logits.stride(1) == 1
