@@ -665,6 +665,10 @@ def plan_pages(lengths: torch.Tensor, new_tokens: torch.Tensor, table: torch.Ten
     return p
 
 
+def _rows(t: torch.Tensor, shape, what: str):
+    assert t.dtype == torch.bfloat16 and tuple(t.shape) == shape and t.stride(1) == 1, f"{what}: bf16 {shape} with unit column stride"
+
+
 def _pools(k_pages: torch.Tensor, v_pages: torch.Tensor, cols: int):
     assert k_pages.dim() == 3 and k_pages.shape == v_pages.shape and k_pages.stride() == v_pages.stride() and k_pages.dtype == v_pages.dtype, "pools of one shape, layout and type"
     assert k_pages.shape[2] == cols and k_pages.stride(2) == 1, f"pools: [n_pages, page_size, {cols}] with unit column stride"
@@ -688,8 +692,8 @@ def attention_decode_paged(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torc
     """Attention of one new token per request over the request's own length of cached tokens (its own among them). q bf16 [B, n_heads * head_dim], pools bf16
     [n_pages, page_size, n_kv_heads * head_dim], table int32 [B, width], lengths int32 [B] on the device (0: zeros). Returns bf16 [B, n_heads * head_dim]. bad (int32 [1]) is set to 1
     where a page lies outside the pool (its tokens are left out) or a length outside the table."""
-    _mat(q, n_heads * head_dim)
-    B = q.shape[0]
+    cols, B = n_heads * head_dim, q.shape[0]
+    _rows(q, (B, cols), "q")
     _pools(k_pages, v_pages, n_kv_heads * head_dim)
     assert k_pages.dtype == torch.bfloat16, "pools: bf16"
     assert table.dtype == torch.int32 and table.dim() == 2 and table.shape[0] == B and table.stride(1) == 1, "table: int32 [B, width] with unit column stride"
@@ -697,8 +701,8 @@ def attention_decode_paged(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torc
     if bad is not None:
         _int32(bad, (1,), "bad")
     if out is None:
-        out = torch.empty(B, n_heads * head_dim, dtype=torch.bfloat16, device=q.device)
-    assert _mat(out, n_heads * head_dim).shape[0] == B
+        out = torch.empty(B, cols, dtype=torch.bfloat16, device=q.device)
+    _rows(out, (B, cols), "out")
     P.need_here(q, k_pages, v_pages, table, lengths, out, bad)
     nbytes = int(P.lib().plz_attn_decode_paged_ws_bytes(n_heads, n_kv_heads, head_dim))
     ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
