@@ -17,7 +17,7 @@
 namespace plz {
 namespace {
 
-constexpr int kTok = 16;                 // tokens of a step
+constexpr int kSwitch = 2;               // steps that the change to another head counts on the line
 constexpr float kGrow = 8.f;             // exponents (base 2) that a maximum may grow before the reference moves
 constexpr float kLog2e = 1.4426950408889634f;
 
@@ -29,7 +29,7 @@ struct PagedParams {
     const int* lengths;
     __nv_bfloat16* out; long long ldo;
     int* bad;
-    float* parts; int4* heads;           // workspace: two parts per CTA; {request, item in it, last CTA of the head that goes on} per CTA
+    float* parts; int4* heads;           // workspace: parts, two of every CTA and one of each of its warps; {request, item in it, last CTA} of the head that goes on from every CTA
     int B, width, page, n_pages, Hq, Hkv, G, blocks, items;   // blocks of 16 query heads per key / value head, items = Hkv * blocks
     int shift;                           // log2(page), or -1
     float scale_log2e;
@@ -39,6 +39,7 @@ __device__ __forceinline__ float ex2f(float x) { float y; asm("ex2.approx.ftz.f3
 __device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool ok) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(ok ? 16 : 0) : "memory");
 }
+__device__ __forceinline__ void copy4(uint32_t dst, const void* src) { asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory"); }
 __device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
 __device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
@@ -54,396 +55,480 @@ __device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uin
 }
 
 // tokens of a request that are attended to
-__device__ __forceinline__ int tokens_of(const PagedParams& p, int b) {
+__device__ __forceinline__ int tokens_of(const PagedParams& p, int len) {
     const long long room = (long long)p.width * p.page;
-    const int len = p.lengths[b];
     return len < 0 ? 0 : (long long)len > room ? (int)room : len;
 }
 
-// a place on the line of steps
+// a place on the line of steps, and how much of a warp's stretch is left from there on
+template <int TOK>
 struct Place {
     int b, item, t, n, len;     // request, item in it, step in the item, steps of the request's items, its tokens
-    __device__ __forceinline__ void open(const PagedParams& p) { len = tokens_of(p, b); n = (len + kTok - 1) / kTok; }
-    __device__ __forceinline__ void next(const PagedParams& p) {
-        if (++t < n) return;
+    int left, ahead;            // ahead: the next request's length, asked for when this one was opened
+    __device__ __forceinline__ void open(const PagedParams& p, int length) {
+        len = tokens_of(p, length);
+        n = (len + TOK - 1) / TOK;
+        ahead = b + 1 < p.B ? p.lengths[b + 1] : 0;
+    }
+    __device__ __forceinline__ void next_item(const PagedParams& p) {
         t = 0;
         if (++item < p.items) return;
         item = 0;
-        do { ++b; if (b < p.B) open(p); } while (b < p.B && n == 0);
+        do {
+            if (++b >= p.B) { left = 0; return; }
+            open(p, ahead);
+        } while (n == 0);
+    }
+    __device__ __forceinline__ void next(const PagedParams& p) {
+        --left;
+        if (++t < n) return;
+        left -= kSwitch;
+        if (left > 0) next_item(p);
     }
 };
 
-template <int D_, int GP_, int NW_, int NST_>
+template <int D_, int GP_, int TOK_, int NW_, int NST_>
 struct Cfg {
-    static constexpr int D = D_, GP = GP_, NW = NW_, NST = NST_;
-    static constexpr int kStage = 2 * kTok * D * 2;                 // bytes of a step: keys, then values
+    static constexpr int D = D_, GP = GP_, TOK = TOK_, NW = NW_, NST = NST_;
+    static constexpr int kTile = TOK * D * 2;                       // bytes of a step's keys, or values
+    static constexpr int kStage = 2 * kTile;
     static constexpr int kPitch = D + 4;                            // floats between rows of a part: D sums, maximum, sum of weights
-    static constexpr int kPart = GP * kPitch * 4;
-    static constexpr int kWarp = NST * kStage + kPart;              // a warp's shared memory: ring, its first part; its last part takes the ring's place
+    static constexpr int kPart = GP * kPitch;                       // floats
+    static constexpr int kWarp = NST * kStage;                      // a warp's shared memory: its ring; the part that it ends with takes the ring's place
     static constexpr int kSmem = NW * kWarp;
-    static_assert(kPart <= NST * kStage, "the last part lies in the ring");
+    static_assert(kPart * 4 <= kWarp, "the last part lies in the ring");
 };
-struct PartMeta { int b, item, flags, rest; };                      // flags 1: valid, 2: holds the head's first step, 4: holds its last; rest: steps behind it
-struct Start { int b; long long off; };
+struct PartMeta { int b, item, flags, rest; };      // flags 1: valid, 2: holds the head's first step, 4: holds its last; rest: steps behind it
 
 template <typename C>
 __global__ void __launch_bounds__(C::NW * 32, 1)
 paged_attn_kernel(const PagedParams p) {
-    constexpr int D = C::D, GP = C::GP, NW = C::NW, NST = C::NST, NR = GP / 8, KS = D / 16, CH = D / 8, ROWS = 32 / CH > 0 ? 32 / CH : 1;
+    constexpr int D = C::D, GP = C::GP, TOK = C::TOK, NW = C::NW, NST = C::NST, NR = GP / 8, KS = D / 16, NT = TOK / 8, CH = D / 8, ROWS = 32 / CH;
     extern __shared__ __align__(128) uint8_t smem[];
-    __shared__ long long sm_sum[NW];
-    __shared__ Start sm_start[NW];
+    __shared__ long long sm_first[NW * 32], sm_sum[NW];      // sums ahead of every thread's requests in its warp, of the warps
     __shared__ PartMeta sm_meta[NW][2];
-    __shared__ uint32_t sm_mask[NW][NST];
+    __shared__ int4 sm_step[NW][2 * NST];           // {request, item, step, tokens} of the steps that are seen
+    __shared__ int sm_page[NW][NST][TOK];           // and the pages of their tokens
+    __shared__ uint32_t sm_mask[NW][NST];           // which tokens of a step that was asked for count
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, cta = blockIdx.x, ctas = gridDim.x;
     pdl_launch_dependents();
     pdl_wait();
 
-    // ---- the line, and where this CTA's warps begin on it
+    // ---- the line, and where this warp begins on it: a request is items * (steps + kSwitch) long, one without tokens 0
+    auto steps_of = [&](int b) { return (tokens_of(p, p.lengths[b]) + TOK - 1) / TOK; };
     const int per = (p.B + NW * 32 - 1) / (NW * 32), r0 = min(p.B, tid * per), r1 = min(p.B, r0 + per);
     long long mine = 0;
-    for (int b = r0; b < r1; ++b) mine += (tokens_of(p, b) + kTok - 1) / kTok;
+    bool empty = false;
+    for (int b = r0; b < r1; ++b) {
+        const int n = steps_of(b);
+        mine += n ? n + kSwitch : 0;
+        empty |= n == 0;
+    }
     long long upto = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
         const long long u = __shfl_up_sync(0xFFFFFFFFu, upto, o);
         if (lane >= o) upto += u;
     }
+    sm_first[tid] = upto - mine;
     if (lane == 31) sm_sum[warp] = upto;
     if (lane < 2) sm_meta[warp][lane].flags = 0;
-    __syncthreads();
-    long long total = 0;
+    empty = __syncthreads_or(empty);
+    // lane w: the sum of the warps ahead of w; lane NW: all
+    long long ahead = 0;
 #pragma unroll
-    for (int w = 0; w < NW; ++w) {
-        if (w < warp) upto += sm_sum[w];
-        total += sm_sum[w];
-    }
-    total *= p.items;
-    const int act = (int)min((long long)ctas, (total + NW - 1) / NW);     // CTAs at work: each has a step at least
-    if (cta < act) {
-        const long long W = (long long)act * NW, first = (upto - mine) * p.items, last = upto * p.items;
-        if (mine > 0) {
-            for (int w = 0; w < NW; ++w) {
-                const long long s = total * (cta * NW + w) / W;
-                if (s < first || s >= last) continue;
-                long long at = first;
-                int b = r0, n;
-                for (;; ++b) {
-                    n = (tokens_of(p, b) + kTok - 1) / kTok;
-                    if (s < at + (long long)n * p.items) break;
-                    at += (long long)n * p.items;
-                }
-                sm_start[w].b = b;
-                sm_start[w].off = s - at;
-            }
+    for (int w = 0; w < NW; ++w) ahead += w < lane ? sm_sum[w] : 0;
+    const long long total = __shfl_sync(0xFFFFFFFFu, ahead, NW) * p.items;
+    // every warp's stretch, and who is at work: CTA c from the places c * NW * stretch on
+    const int W = ctas * NW;
+    const long long stretch = max(total <= 0x7FFFFFFF - W ? (long long)(((int)total + W - 1) / W) : (total + W - 1) / W, 1ll);
+    const long long begin = (cta * NW + warp) * stretch;
+    Place<TOK> eye;
+    eye.left = (int)min(total - begin, stretch);
+    if (eye.left > 0) {
+        // the thread whose requests hold that place, then the request
+        const int group = __popc(__ballot_sync(0xFFFFFFFFu, lane < NW && ahead * p.items <= begin)) - 1;
+        const long long base = __shfl_sync(0xFFFFFFFFu, ahead, group);
+        const int who = group * 32 + __popc(__ballot_sync(0xFFFFFFFFu, (base + sm_first[group * 32 + lane]) * p.items <= begin)) - 1;
+        long long off = begin - (base + sm_first[who]) * p.items;
+        eye.b = who * per;
+        while (true) {
+            eye.open(p, p.lengths[eye.b]);
+            const long long size = eye.n ? (long long)(eye.n + kSwitch) * p.items : 0;
+            if (off < size) break;
+            off -= size;
+            ++eye.b;
+        }
+        const int one = eye.n + kSwitch;
+        eye.item = off <= 0x7FFFFFFF ? (int)off / one : (int)(off / one);
+        eye.t = (int)(off - (long long)eye.item * one);
+        if (eye.t >= eye.n) {
+            eye.left -= one - eye.t;
+            if (eye.left > 0) eye.next_item(p);
         }
     }
-    __syncthreads();
 
-    const uint32_t ring = smem_u32(smem) + warp * C::kWarp;
-    float* const part0 = reinterpret_cast<float*>(smem + warp * C::kWarp + NST * C::kStage);
-    float* const part1 = reinterpret_cast<float*>(smem + warp * C::kWarp);
-    if (cta < act) {
-        const long long W = (long long)act * NW, s0 = total * (cta * NW + warp) / W, s1 = total * (cta * NW + warp + 1) / W;
-        long long todo = s1 - s0;
-        if (todo > 0) {
-            Place at;
-            at.b = sm_start[warp].b;
-            at.open(p);
-            at.item = (int)(sm_start[warp].off / at.n);
-            at.t = (int)(sm_start[warp].off - (long long)at.item * at.n);
-            Place ahead = at;
-            long long to_ask = todo;
-            // the lane's token of the step that is asked for next: page and row in it
-            int pg = -1, in = 0;
-            auto look = [&]() {
-                const int tok = ahead.t * kTok + (lane & 15);
-                pg = -1;
-                if (to_ask > 0 && tok < ahead.len) {
-                    const int j = p.shift >= 0 ? tok >> p.shift : tok / p.page;
-                    in = tok - j * p.page;
-                    pg = p.table[(long long)ahead.b * p.ldt + j];
-                }
-            };
-            auto ask = [&](int slot) {
-                if (to_ask > 0) {
-                    const bool in_len = ahead.t * kTok + (lane & 15) < ahead.len, ok = in_len && (unsigned)pg < (unsigned)p.n_pages;
-                    if (in_len && !ok && p.bad) *p.bad = 1;
-                    const uint32_t mask = __ballot_sync(0xFFFFFFFFu, ok) & 0xFFFFu;
-                    if (lane == 0) sm_mask[warp][slot] = mask;
-                    const unsigned off = ok ? (unsigned)pg * p.page16 + (unsigned)in * p.tok16 : 0u;
-                    const int head = ahead.item / p.blocks, c0 = lane % CH;
-                    const uint32_t dst = ring + slot * C::kStage;
+    uint8_t* const mine_smem = smem + warp * C::kWarp;
+    const uint32_t ring = smem_u32(mine_smem);
+    if (eye.left > 0) {
+        int seen = 0;                    // steps whose pages are asked for; all of the stretch's in the end
+        const int lt = lane & (TOK - 1);
+        auto see = [&]() {
+            if (eye.left <= 0) return;
+            if (lane == 0) sm_step[warp][seen % (2 * NST)] = make_int4(eye.b, eye.item, eye.t, eye.len);
+            const int tok = eye.t * TOK + lt;
+            if (lane < TOK && tok < eye.len)
+                copy4(smem_u32(&sm_page[warp][seen % NST][lt]), p.table + (long long)eye.b * p.ldt + (p.shift >= 0 ? tok >> p.shift : tok / p.page));
+            ++seen;
+            eye.next(p);
+        };
+        auto ask = [&](int step) {
+            if (step >= seen) return;
+            const int slot = step % NST;
+            const int4 st = sm_step[warp][step % (2 * NST)];
+            const int tok = st.z * TOK + lt, pg = sm_page[warp][slot][lt];
+            const bool in_len = tok < st.w, ok = in_len && (unsigned)pg < (unsigned)p.n_pages;
+            if (in_len && !ok && p.bad) *p.bad = 1;
+            const uint32_t mask = __ballot_sync(0xFFFFFFFFu, ok);
+            if (lane == 0) sm_mask[warp][slot] = mask;
+            const int in = p.shift >= 0 ? tok & (p.page - 1) : tok % p.page;
+            const unsigned off = ok ? (unsigned)pg * p.page16 + (unsigned)in * p.tok16 : 0u;
+            const int head = p.blocks == 1 ? st.y : st.y / p.blocks, c0 = lane % CH;
+            const __nv_bfloat16 *kb = p.k + head * D + c0 * 8, *vb = p.v + head * D + c0 * 8;
+            const uint32_t dst = ring + slot * C::kStage;
 #pragma unroll
-                    for (int i = 0; i < kTok / ROWS; ++i) {
-                        const int row = i * ROWS + lane / CH;
-                        const unsigned o = __shfl_sync(0xFFFFFFFFu, off, row);
-                        const bool good = (mask >> row) & 1u;
-                        const size_t src = (size_t)o * 8 + head * D + c0 * 8;
-                        const uint32_t d = dst + row * (D * 2) + ((c0 ^ (row & 7)) << 4);
-                        copy16(d, p.k + src, good);
-                        copy16(d + kTok * D * 2, p.v + src, good);
-                    }
-                    if (--to_ask > 0) ahead.next(p);
-                    look();
-                }
-                copy_commit();
-            };
-            look();
-#pragma unroll
-            for (int i = 0; i < NST; ++i) ask(i);
+            for (int i = 0; i < TOK / ROWS; ++i) {
+                const int row = i * ROWS + lane / CH;
+                const unsigned o = __shfl_sync(0xFFFFFFFFu, off, row);
+                const bool good = (mask >> row) & 1u;
+                const uint32_t d = dst + row * (D * 2) + ((c0 ^ (row & 7)) << 4);
+                copy16(d, kb + (size_t)o * 8, good);
+                copy16(d + C::kTile, vb + (size_t)o * 8, good);
+            }
+        };
+        // pages are asked for 2 NST steps ahead, keys and values NST: a group is one step's keys and values and a later one's pages
+#pragma unroll 1
+        for (int i = 0; i < NST; ++i) see();
+        copy_commit();
+        copy_wait<0>();
+        __syncwarp();
+#pragma unroll 1
+        for (int i = 0; i < NST; ++i) { ask(i); see(); copy_commit(); }
 
-            uint32_t qf[KS][2 * NR];
-            float acc[D / 8][4], m[NR], l[NR];
-            bool fresh = true, from_start = at.t == 0;
-            int slot = 0, which = 0;
-            const int g = lane >> 2, c2 = (lane & 3) * 2;
-            while (true) {
-                const int hk = at.item / p.blocks, h0 = (at.item - hk * p.blocks) * 16, heads = min(p.G - h0, 16);
-                if (fresh) {
-                    fresh = false;
-                    const __nv_bfloat16* qr = p.q + (long long)at.b * p.ldq + (long long)(hk * p.G + h0) * D + c2;
+        uint32_t qf[KS][2 * NR];
+        float acc[D / 8][4], m[NR], l[NR];
+        bool fresh = true, from_start = false;
+        const int g = lane >> 2, c2 = (lane & 3) * 2;
+#pragma unroll 1
+        for (int step = 0, slot = 0;; ++step) {
+            const int4 st = sm_step[warp][step % (2 * NST)];
+            const int hk = p.blocks == 1 ? st.y : st.y / p.blocks, h0 = (st.y - hk * p.blocks) * 16, heads = min(p.G - h0, 16);
+            if (fresh) {
+                fresh = false;
+                from_start = st.z == 0;
+                const __nv_bfloat16* qr = p.q + (long long)st.x * p.ldq + (long long)(hk * p.G + h0) * D + c2;
 #pragma unroll
-                    for (int ks = 0; ks < KS; ++ks)
+                for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
-                        for (int r = 0; r < NR; ++r)
+                    for (int r = 0; r < NR; ++r)
 #pragma unroll
-                            for (int h = 0; h < 2; ++h)
-                                qf[ks][r + NR * h] = g + 8 * r < heads ? *reinterpret_cast<const uint32_t*>(qr + (long long)(g + 8 * r) * D + ks * 16 + h * 8) : 0u;
+                        for (int h = 0; h < 2; ++h)
+                            qf[ks][r + NR * h] = g + 8 * r < heads ? *reinterpret_cast<const uint32_t*>(qr + (long long)(g + 8 * r) * D + ks * 16 + h * 8) : 0u;
 #pragma unroll
-                    for (int n = 0; n < D / 8; ++n)
+                for (int n = 0; n < D / 8; ++n)
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) acc[n][e] = 0.f;
+                    for (int e = 0; e < 4; ++e) acc[n][e] = 0.f;
 #pragma unroll
-                    for (int r = 0; r < NR; ++r) { m[r] = -INFINITY; l[r] = 0.f; }
-                }
-                copy_wait<NST - 1>();
-                __syncwarp();
-                const uint32_t kt = ring + slot * C::kStage, vt = kt + kTok * D * 2;
-                const uint32_t mask = sm_mask[warp][slot];
-                float s[2][4];
+                for (int r = 0; r < NR; ++r) { m[r] = -INFINITY; l[r] = 0.f; }
+            }
+            copy_wait<NST - 1>();
+            __syncwarp();
+            const uint32_t kt = ring + slot * C::kStage, vt = kt + C::kTile;
+            const uint32_t mask = sm_mask[warp][slot];
+            float s[NT][4];
 #pragma unroll
-                for (int n = 0; n < 2; ++n)
+            for (int n = 0; n < NT; ++n)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) s[n][e] = 0.f;
-                {
-                    const int row = (lane & 7) + ((lane >> 4) << 3), odd = (lane >> 3) & 1;
-                    const uint32_t base = kt + row * (D * 2);
+                for (int e = 0; e < 4; ++e) s[n][e] = 0.f;
+            {
+                const int row = (lane & 7) + ((lane >> 4) << 3), upper = (lane >> 3) & 1;
+                const uint32_t base = kt + row * (D * 2);
 #pragma unroll
-                    for (int ks = 0; ks < KS; ++ks) {
+                for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+                    for (int n = 0; n < NT; n += 2) {
                         uint32_t b[4];
-                        ldm4(b, base + (((2 * ks + odd) ^ (lane & 7)) << 4));
+                        ldm4(b, base + n * 8 * (D * 2) + (((2 * ks + upper) ^ (lane & 7)) << 4));
                         if constexpr (NR == 1) {
-                            mma(s[0], qf[ks][0], 0u, qf[ks][1], 0u, b[0], b[1]);
-                            mma(s[1], qf[ks][0], 0u, qf[ks][1], 0u, b[2], b[3]);
+                            mma(s[n], qf[ks][0], 0u, qf[ks][1], 0u, b[0], b[1]);
+                            mma(s[n + 1], qf[ks][0], 0u, qf[ks][1], 0u, b[2], b[3]);
                         } else {
-                            mma(s[0], qf[ks][0], qf[ks][1], qf[ks][2], qf[ks][3], b[0], b[1]);
-                            mma(s[1], qf[ks][0], qf[ks][1], qf[ks][2], qf[ks][3], b[2], b[3]);
+                            mma(s[n], qf[ks][0], qf[ks][1], qf[ks][2], qf[ks][3], b[0], b[1]);
+                            mma(s[n + 1], qf[ks][0], qf[ks][1], qf[ks][2], qf[ks][3], b[2], b[3]);
                         }
                     }
-                }
-                // scaled scores, maxima of the rows over the tokens that count
-                float top[NR];
+            }
+            // scaled scores, maxima of the rows over the tokens that count
+            float top[NR];
+#pragma unroll
+            for (int r = 0; r < NR; ++r) {
+                top[r] = -INFINITY;
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        s[n][2 * r + e] *= p.scale_log2e;
+                        if ((mask >> (n * 8 + c2 + e)) & 1u) top[r] = fmaxf(top[r], s[n][2 * r + e]);
+                    }
+                top[r] = fmaxf(top[r], __shfl_xor_sync(0xFFFFFFFFu, top[r], 1));
+                top[r] = fmaxf(top[r], __shfl_xor_sync(0xFFFFFFFFu, top[r], 2));
+            }
+            bool moves = false;
+#pragma unroll
+            for (int r = 0; r < NR; ++r) moves |= top[r] > m[r] + kGrow;       // m = -inf: any score moves it
+            if (__any_sync(0xFFFFFFFFu, moves)) {
+                float f[NR];
 #pragma unroll
                 for (int r = 0; r < NR; ++r) {
-                    top[r] = -INFINITY;
-#pragma unroll
-                    for (int n = 0; n < 2; ++n)
-#pragma unroll
-                        for (int e = 0; e < 2; ++e) {
-                            s[n][2 * r + e] *= p.scale_log2e;
-                            if ((mask >> (n * 8 + c2 + e)) & 1u) top[r] = fmaxf(top[r], s[n][2 * r + e]);
-                        }
-                    top[r] = fmaxf(top[r], __shfl_xor_sync(0xFFFFFFFFu, top[r], 1));
-                    top[r] = fmaxf(top[r], __shfl_xor_sync(0xFFFFFFFFu, top[r], 2));
+                    const float to = fmaxf(m[r], top[r]);
+                    f[r] = m[r] == to ? 1.f : ex2f(m[r] - to);
+                    m[r] = to;
+                    l[r] *= f[r];
                 }
-                bool moves = false;
 #pragma unroll
-                for (int r = 0; r < NR; ++r) moves |= top[r] > m[r] + kGrow;       // m = -inf: any score moves it
-                if (__any_sync(0xFFFFFFFFu, moves)) {
-                    float f[NR];
-#pragma unroll
-                    for (int r = 0; r < NR; ++r) {
-                        const float to = fmaxf(m[r], top[r]);
-                        f[r] = m[r] == to ? 1.f : ex2f(m[r] - to);
-                        m[r] = to;
-                        l[r] *= f[r];
-                    }
-#pragma unroll
-                    for (int n = 0; n < D / 8; ++n) {
-                        acc[n][0] *= f[0]; acc[n][1] *= f[0];
-                        acc[n][2] *= f[NR - 1]; acc[n][3] *= f[NR - 1];
-                    }
+                for (int n = 0; n < D / 8; ++n) {
+                    acc[n][0] *= f[0]; acc[n][1] *= f[0];
+                    acc[n][2] *= f[NR - 1]; acc[n][3] *= f[NR - 1];
                 }
-                uint32_t hi[2][NR], lo[2][NR];
+            }
+            uint32_t hi[NT][NR], lo[NT][NR];
 #pragma unroll
-                for (int r = 0; r < NR; ++r) {
-                    const float ref = m[r] == -INFINITY ? 0.f : m[r];
+            for (int r = 0; r < NR; ++r) {
+                const float ref = m[r] == -INFINITY ? 0.f : m[r];
 #pragma unroll
-                    for (int n = 0; n < 2; ++n) {
-                        float w[2];
+                for (int n = 0; n < NT; ++n) {
+                    float w[2];
 #pragma unroll
-                        for (int e = 0; e < 2; ++e) {
-                            w[e] = (mask >> (n * 8 + c2 + e)) & 1u ? ex2f(s[n][2 * r + e] - ref) : 0.f;
-                            l[r] += w[e];
-                        }
-                        hi[n][r] = pack_bf16x2(w[0], w[1]);
-                        lo[n][r] = pack_bf16x2(w[0] - __uint_as_float(hi[n][r] << 16), w[1] - __uint_as_float(hi[n][r] & 0xFFFF0000u));
+                    for (int e = 0; e < 2; ++e) {
+                        w[e] = (mask >> (n * 8 + c2 + e)) & 1u ? ex2f(s[n][2 * r + e] - ref) : 0.f;
+                        l[r] += w[e];
                     }
+                    hi[n][r] = pack_bf16x2(w[0], w[1]);
+                    lo[n][r] = pack_bf16x2(w[0] - __uint_as_float(hi[n][r] << 16), w[1] - __uint_as_float(hi[n][r] & 0xFFFF0000u));
                 }
-                {
-                    const int row = (lane & 7) + (((lane >> 3) & 1) << 3), odd = lane >> 4;
-                    const uint32_t base = vt + row * (D * 2);
+            }
+            {
+                const int row = (lane & 7) + (((lane >> 3) & 1) << 3), upper = lane >> 4;
+                const uint32_t base = vt + row * (D * 2);
+#pragma unroll
+                for (int n = 0; n < NT; n += 2)
 #pragma unroll
                     for (int j = 0; j < D / 16; ++j) {
                         uint32_t b[4];
-                        ldm4t(b, base + (((2 * j + odd) ^ (lane & 7)) << 4));
+                        ldm4t(b, base + n * 8 * (D * 2) + (((2 * j + upper) ^ (lane & 7)) << 4));
                         if constexpr (NR == 1) {
-                            mma(acc[2 * j], hi[0][0], lo[0][0], hi[1][0], lo[1][0], b[0], b[1]);
-                            mma(acc[2 * j + 1], hi[0][0], lo[0][0], hi[1][0], lo[1][0], b[2], b[3]);
+                            mma(acc[2 * j], hi[n][0], lo[n][0], hi[n + 1][0], lo[n + 1][0], b[0], b[1]);
+                            mma(acc[2 * j + 1], hi[n][0], lo[n][0], hi[n + 1][0], lo[n + 1][0], b[2], b[3]);
                         } else {
-                            mma(acc[2 * j], hi[0][0], hi[0][1], hi[1][0], hi[1][1], b[0], b[1]);
-                            mma(acc[2 * j + 1], hi[0][0], hi[0][1], hi[1][0], hi[1][1], b[2], b[3]);
-                            mma(acc[2 * j], lo[0][0], lo[0][1], lo[1][0], lo[1][1], b[0], b[1]);
-                            mma(acc[2 * j + 1], lo[0][0], lo[0][1], lo[1][0], lo[1][1], b[2], b[3]);
+                            mma(acc[2 * j], hi[n][0], hi[n][1], hi[n + 1][0], hi[n + 1][1], b[0], b[1]);
+                            mma(acc[2 * j + 1], hi[n][0], hi[n][1], hi[n + 1][0], hi[n + 1][1], b[2], b[3]);
+                            mma(acc[2 * j], lo[n][0], lo[n][1], lo[n + 1][0], lo[n + 1][1], b[0], b[1]);
+                            mma(acc[2 * j + 1], lo[n][0], lo[n][1], lo[n + 1][0], lo[n + 1][1], b[2], b[3]);
                         }
                     }
+            }
+            const bool over = step + 1 == seen, done = (st.z + 1) * TOK >= st.w;
+            __syncwarp();
+            ask(step + NST);
+            see();
+            copy_commit();
+            slot = slot + 1 == NST ? 0 : slot + 1;
+            if (done || over) {
+                // rows r of this lane: query head g + 8 r
+#pragma unroll
+                for (int r = 0; r < NR; ++r) {
+                    l[r] += __shfl_xor_sync(0xFFFFFFFFu, l[r], 1);
+                    l[r] += __shfl_xor_sync(0xFFFFFFFFu, l[r], 2);
                 }
-                __syncwarp();
-                ask(slot);
-                slot = slot + 1 == NST ? 0 : slot + 1;
-                --todo;
-                const bool done = at.t + 1 == at.n;
-                if (done || todo == 0) {
-                    // rows r of this lane: query head g + 8 r
+                if constexpr (NR == 1) {
+#pragma unroll
+                    for (int n = 0; n < D / 8; ++n) { acc[n][0] += acc[n][2]; acc[n][1] += acc[n][3]; }
+                }
+                if (done && from_start) {
 #pragma unroll
                     for (int r = 0; r < NR; ++r) {
-                        l[r] += __shfl_xor_sync(0xFFFFFFFFu, l[r], 1);
-                        l[r] += __shfl_xor_sync(0xFFFFFFFFu, l[r], 2);
+                        if (g + 8 * r >= heads) continue;
+                        const float inv = 1.f / l[r];
+                        __nv_bfloat16* o = p.out + (long long)st.x * p.ldo + (long long)(hk * p.G + h0 + g + 8 * r) * D + c2;
+#pragma unroll
+                        for (int n = 0; n < D / 8; ++n) *reinterpret_cast<uint32_t*>(o + n * 8) = pack_bf16x2(acc[n][2 * r] * inv, acc[n][2 * r + 1] * inv);
                     }
-                    if constexpr (NR == 1) {
+                } else {
+                    // the part that a warp ends with goes to the place of its ring, into which nothing comes any more, the one that it began with, while the ring is at work, to the workspace
+                    float* const part = over ? reinterpret_cast<float*>(mine_smem) : p.parts + ((size_t)cta * (2 + NW) + 2 + warp) * C::kPart;
 #pragma unroll
-                        for (int n = 0; n < D / 8; ++n) { acc[n][0] += acc[n][2]; acc[n][1] += acc[n][3]; }
+                    for (int r = 0; r < NR; ++r) {
+                        float* row = part + (g + 8 * r) * C::kPitch;
+#pragma unroll
+                        for (int n = 0; n < D / 8; ++n) *reinterpret_cast<float2*>(row + n * 8 + c2) = make_float2(acc[n][2 * r], acc[n][2 * r + 1]);
+                        if (c2 == 0) *reinterpret_cast<float2*>(row + D) = make_float2(m[r], l[r]);
                     }
-                    if (done && from_start) {
-#pragma unroll
-                        for (int r = 0; r < NR; ++r) {
-                            if (g + 8 * r >= heads) continue;
-                            const float inv = 1.f / l[r];
-                            __nv_bfloat16* o = p.out + (long long)at.b * p.ldo + (long long)(hk * p.G + h0 + g + 8 * r) * D + c2;
-#pragma unroll
-                            for (int n = 0; n < D / 8; ++n) *reinterpret_cast<uint32_t*>(o + n * 8) = pack_bf16x2(acc[n][2 * r] * inv, acc[n][2 * r + 1] * inv);
-                        }
-                    } else {
-                        // a last part comes when nothing is left to arrive in the ring
-                        which = from_start ? 1 : 0;
-                        if (which) { copy_wait<0>(); __syncwarp(); }
-                        float* part = which ? part1 : part0;
-#pragma unroll
-                        for (int r = 0; r < NR; ++r) {
-                            float* row = part + (g + 8 * r) * C::kPitch;
-#pragma unroll
-                            for (int n = 0; n < D / 8; ++n) *reinterpret_cast<float2*>(row + n * 8 + c2) = make_float2(acc[n][2 * r], acc[n][2 * r + 1]);
-                            if (c2 == 0) { row[D] = m[r]; row[D + 1] = l[r]; }
-                        }
-                        if (lane == 0) sm_meta[warp][which] = PartMeta{at.b, at.item, 1 | (from_start ? 2 : 0) | (done ? 4 : 0), at.n - at.t - 1};
-                    }
-                    if (todo == 0) break;
-                    fresh = from_start = true;
+                    if (lane == 0) sm_meta[warp][over] = PartMeta{st.x, st.y, 1 | (from_start ? 2 : 0) | (done ? 4 : 0), (st.w + TOK - 1) / TOK - st.z - 1};
                 }
-                at.next(p);
+                if (over) break;
+                fresh = true;
             }
-            copy_wait<0>();
         }
+        copy_wait<0>();
     }
     __syncthreads();
 
-    // ---- the parts of this CTA, in order
-    auto part_at = [&](int i) { return reinterpret_cast<const float*>(smem + (i >> 1) * C::kWarp + (i & 1 ? 0 : NST * C::kStage)); };
-    int4 goes_on = make_int4(0, 0, -1, 0);
-    for (int i = 0; i < 2 * NW;) {
-        const PartMeta a = sm_meta[i >> 1][i & 1];
-        if (!(a.flags & 1)) { ++i; continue; }
-        int e = i, flags = a.flags;
-        for (int j = i + 1; j < 2 * NW && !(flags & 4); ++j) {
-            const int f = sm_meta[j >> 1][j & 1].flags;
-            if (f & 1) { e = j; flags |= f; }
+    // ---- the parts of this CTA, in order: those of one head follow one another. A warp takes a head and one of its rows at a time.
+    auto part_at = [&](int i) -> const float* {
+        return i & 1 ? reinterpret_cast<const float*>(smem + (i >> 1) * C::kWarp) : p.parts + ((size_t)cta * (2 + NW) + 2 + (i >> 1)) * C::kPart;
+    };
+    const PartMeta own = lane < 2 * NW ? sm_meta[lane >> 1][lane & 1] : PartMeta{0, 0, 0, 0};
+    const uint32_t valid = __ballot_sync(0xFFFFFFFFu, own.flags & 1), starts = __ballot_sync(0xFFFFFFFFu, (own.flags & 3) == 3) | (valid & -valid);
+    const uint32_t ends = __ballot_sync(0xFFFFFFFFu, (own.flags & 5) == 5), begun = __ballot_sync(0xFFFFFFFFu, (own.flags & 3) == 3);
+    if (tid == (NW - 1) * 32) p.heads[cta] = make_int4(0, 0, -1, 0);
+    int turn = 0;
+    for (uint32_t todo = starts; todo; todo &= todo - 1) {
+        const int i = __ffs(todo) - 1, upper = todo & (todo - 1) ? __ffs(todo & (todo - 1)) - 1 : 32;
+        const uint32_t run = valid & ~((1u << i) - 1u) & (upper == 32 ? 0xFFFFFFFFu : (1u << upper) - 1u);
+        const int e = 31 - __clz(run);
+        const bool first = (begun >> i) & 1u, last = (ends >> e) & 1u;
+        const int b = __shfl_sync(0xFFFFFFFFu, own.b, i), item = __shfl_sync(0xFFFFFFFFu, own.item, i), rest = __shfl_sync(0xFFFFFFFFu, own.rest, e);
+        const int hk = p.blocks == 1 ? item : item / p.blocks, h0 = (item - hk * p.blocks) * 16, heads = min(p.G - h0, 16);
+        if (warp == NW - 1 && lane == 0 && first && !last) {
+            // the head ends `rest` steps behind this CTA's stretches: the CTA that holds the last of them
+            const long long at = (long long)(cta + 1) * NW * stretch + rest - 1, size = NW * stretch;
+            p.heads[cta] = make_int4(b, item, at <= 0x7FFFFFFF ? (int)at / (int)size : (int)(at / size), 0);
         }
-        const int hk = a.item / p.blocks, h0 = (a.item - hk * p.blocks) * 16, heads = min(p.G - h0, 16);
-        const bool whole = (flags & 6) == 6;
-        float* to = p.parts + (size_t)(2 * cta + (flags & 2 ? 1 : 0)) * GP * C::kPitch;
-        for (int x = tid * 4; x < heads * D; x += NW * 128) {
-            const int row = x / D, d = x - row * D;
-            float top = -INFINITY;
-            for (int j = i; j <= e; ++j)
-                if (sm_meta[j >> 1][j & 1].flags & 1) top = fmaxf(top, part_at(j)[row * C::kPitch + D]);
-            float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-            float l = 0.f;
-            for (int j = i; j <= e; ++j) {
-                if (!(sm_meta[j >> 1][j & 1].flags & 1)) continue;
-                const float* part = part_at(j) + row * C::kPitch;
-                const float m = part[D], f = m == top ? 1.f : ex2f(m - top);
-                const float4 v = *reinterpret_cast<const float4*>(part + d);
-                o.x += f * v.x; o.y += f * v.y; o.z += f * v.z; o.w += f * v.w;
-                l += f * part[D + 1];
+        float* const to = p.parts + ((size_t)cta * (2 + NW) + (first ? 1 : 0)) * C::kPart;
+        for (int row = 0; row < heads; ++row, turn = turn + 1 == NW ? 0 : turn + 1) {
+            if (turn != warp) continue;
+            // lane j: part j's maximum and sum of weights
+            float2 ml = make_float2(-INFINITY, 0.f);
+            if ((run >> lane) & 1u) ml = *reinterpret_cast<const float2*>(part_at(lane) + row * C::kPitch + D);
+            float top = ml.x;
+#pragma unroll
+            for (int o = 1; o < 2 * NW; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
+            top = __shfl_sync(0xFFFFFFFFu, top, i);
+            const float f = ml.x == top ? 1.f : ex2f(ml.x - top);
+            float l = (run >> lane) & 1u ? f * ml.y : 0.f;
+#pragma unroll
+            for (int o = 1; o < 2 * NW; o <<= 1) l += __shfl_xor_sync(0xFFFFFFFFu, l, o);
+            l = __shfl_sync(0xFFFFFFFFu, l, i);
+#pragma unroll
+            for (int n = 0; n < (D + 127) / 128; ++n) {
+                const int d = n * 128 + lane * 4;
+                // All parts are asked for ahead of the sum, without branches: what is no part of the run is whatever lies there, and left out. Only few heads have one in the workspace.
+                float4 v[2 * NW];
+                const int at = row * C::kPitch + (d < D ? d : 0);
+#pragma unroll
+                for (int j = 1; j < 2 * NW; j += 2) v[j] = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(smem + (j >> 1) * C::kWarp) + at);
+                if (run & 0x55555555u) {
+#pragma unroll
+                    for (int j = 0; j < 2 * NW; j += 2) v[j] = *reinterpret_cast<const float4*>(p.parts + ((size_t)cta * (2 + NW) + 2 + (j >> 1)) * C::kPart + at);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 2 * NW; j += 2) v[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+                }
+                float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+                for (int j = 0; j < 2 * NW; ++j) {
+                    const float fj = __shfl_sync(0xFFFFFFFFu, f, j);
+                    const bool in = (run >> j) & 1u;
+                    o.x += in ? fj * v[j].x : 0.f; o.y += in ? fj * v[j].y : 0.f; o.z += in ? fj * v[j].z : 0.f; o.w += in ? fj * v[j].w : 0.f;
+                }
+                if (d >= D) continue;
+                if (first && last) {
+                    const float inv = 1.f / l;
+                    *reinterpret_cast<uint2*>(p.out + (long long)b * p.ldo + (long long)(hk * p.G + h0 + row) * D + d) =
+                        make_uint2(pack_bf16x2(o.x * inv, o.y * inv), pack_bf16x2(o.z * inv, o.w * inv));
+                } else {
+                    *reinterpret_cast<float4*>(to + row * C::kPitch + d) = o;
+                }
             }
-            if (whole) {
-                const float inv = 1.f / l;
-                *reinterpret_cast<uint2*>(p.out + (long long)a.b * p.ldo + (long long)(hk * p.G + h0 + row) * D + d) =
-                    make_uint2(pack_bf16x2(o.x * inv, o.y * inv), pack_bf16x2(o.z * inv, o.w * inv));
-            } else {
-                *reinterpret_cast<float4*>(to + row * C::kPitch + d) = o;
-                if (d == 0) { to[row * C::kPitch + D] = top; to[row * C::kPitch + D + 1] = l; }
-            }
+            if (!(first && last) && lane == 0) *reinterpret_cast<float2*>(to + row * C::kPitch + D) = make_float2(top, l);
         }
-        if ((flags & 6) == 2) {
-            // the head ends `rest` steps behind this CTA's stretch: the CTA that holds the last of them
-            const long long end = total * (cta + 1) / act + sm_meta[e >> 1][e & 1].rest;
-            goes_on = make_int4(a.b, a.item, (int)((end * act - 1) / total), 0);
-        }
-        i = e + 1;
     }
-    if (tid == 0) p.heads[cta] = goes_on;
 
-    // ---- requests without tokens
-    for (int b = cta; b < p.B; b += ctas) {
+    // ---- requests without tokens, and lengths that there cannot be
+    for (int b = empty || p.bad ? cta : p.B; b < p.B; b += ctas) {
         const int len = p.lengths[b];
         if (tid == 0 && p.bad && (len < 0 || len > (long long)p.width * p.page)) *p.bad = 1;
-        if (tokens_of(p, b) > 0) continue;
+        if (!empty || tokens_of(p, len) > 0) continue;
         for (int x = tid * 8; x < p.Hq * D; x += NW * 256) *reinterpret_cast<uint4*>(p.out + (long long)b * p.ldo + x) = make_uint4(0u, 0u, 0u, 0u);
     }
 }
 
-// out = (sum_i 2^(m_i - m) o_i) / (sum_i 2^(m_i - m) l_i) over the parts i of a head, m the largest m_i: the second part of this CTA, the first ones of those behind it
+// out = (sum_i 2^(m_i - m) o_i) / (sum_i 2^(m_i - m) l_i) over the parts i of a head, m the largest m_i: the second part of the CTA where the head began, the first ones of those
+// behind it. One block per such CTA and query head of the item; its warps take the parts in turns, all loads of a warp's turn at once, and meet in shared memory.
+// One sequence of 2049 tokens, 18 parts a head: 11 us with a thread per four sums of all heads.
+constexpr int kJoinWarps = 8;
 template <int D>
-__global__ void __launch_bounds__(256)
-paged_join_kernel(const PagedParams p, int gp) {
-    constexpr int kPitch = D + 4;
+__global__ void __launch_bounds__(kJoinWarps * 32)
+paged_join_kernel(const PagedParams p, int part, int per_cta) {
+    constexpr int kPitch = D + 4, N = (D + 127) / 128, kTurn = 4;       // float4s of a lane; parts of a warp's turn
+    __shared__ float4 sm_o[kJoinWarps][N][32];
+    __shared__ float2 sm_ml[kJoinWarps];
     pdl_launch_dependents();
     pdl_wait();
-    const int cta = blockIdx.x;
+    const int cta = blockIdx.x, row = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int4 h = p.heads[cta];
     if (h.z <= cta) return;
-    const int hk = h.y / p.blocks, h0 = (h.y - hk * p.blocks) * 16, heads = min(p.G - h0, 16);
-    const size_t step = (size_t)2 * gp * kPitch;
-    for (int x = threadIdx.x * 4; x < heads * D; x += 1024) {
-        const int row = x / D, d = x - row * D;
-        const float* const first = p.parts + (size_t)(2 * cta + 1) * gp * kPitch + row * kPitch;
-        const float* const rest = p.parts + (size_t)2 * cta * gp * kPitch + row * kPitch;      // CTA cta + i: i steps on
-        float top = first[D];
-        for (int i = 1; i <= h.z - cta; ++i) top = fmaxf(top, rest[i * step + D]);
-        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-        float l = 0.f;
-#pragma unroll 4
-        for (int i = 0; i <= h.z - cta; ++i) {
+    const int hk = h.y / p.blocks, h0 = (h.y - hk * p.blocks) * 16, count = h.z - cta + 1;
+    if (row >= min(p.G - h0, 16)) return;
+    const size_t step = (size_t)per_cta * part;
+    const float* const rest = p.parts + cta * step + row * kPitch;      // CTA cta + i: i steps on
+    const float* const first = rest + part;
+    float top = -INFINITY, l = 0.f;
+    float4 o[N];
+#pragma unroll
+    for (int n = 0; n < N; ++n) o[n] = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int i0 = warp; i0 < count; i0 += kJoinWarps * kTurn) {
+        float2 ml[kTurn];
+        float4 v[kTurn][N];
+#pragma unroll
+        for (int t = 0; t < kTurn; ++t) {
+            const int i = i0 + t * kJoinWarps;
+            if (i >= count) break;
             const float* part = i ? rest + i * step : first;
-            const float m = part[D], f = m == top ? 1.f : ex2f(m - top);
-            const float4 v = *reinterpret_cast<const float4*>(part + d);
-            o.x += f * v.x; o.y += f * v.y; o.z += f * v.z; o.w += f * v.w;
-            l += f * part[D + 1];
+            ml[t] = *reinterpret_cast<const float2*>(part + D);
+#pragma unroll
+            for (int n = 0; n < N; ++n)
+                if (n * 128 + lane * 4 < D) v[t][n] = *reinterpret_cast<const float4*>(part + n * 128 + lane * 4);
         }
-        const float inv = 1.f / l;
-        *reinterpret_cast<uint2*>(p.out + (long long)h.x * p.ldo + (long long)(hk * p.G + h0 + row) * D + d) = make_uint2(pack_bf16x2(o.x * inv, o.y * inv), pack_bf16x2(o.z * inv, o.w * inv));
+#pragma unroll
+        for (int t = 0; t < kTurn; ++t) {
+            if (i0 + t * kJoinWarps >= count) break;
+            const float to = fmaxf(top, ml[t].x), f = top == to ? 1.f : ex2f(top - to), g = ml[t].x == to ? 1.f : ex2f(ml[t].x - to);
+            top = to;
+            l = l * f + ml[t].y * g;
+#pragma unroll
+            for (int n = 0; n < N; ++n) {
+                o[n].x = o[n].x * f + v[t][n].x * g; o[n].y = o[n].y * f + v[t][n].y * g;
+                o[n].z = o[n].z * f + v[t][n].z * g; o[n].w = o[n].w * f + v[t][n].w * g;
+            }
+        }
+    }
+#pragma unroll
+    for (int n = 0; n < N; ++n) sm_o[warp][n][lane] = o[n];
+    if (lane == 0) sm_ml[warp] = make_float2(top, l);
+    __syncthreads();
+    for (int x = threadIdx.x; x < D; x += kJoinWarps * 32) {
+        float m = -INFINITY, sum = 0.f, w = 0.f;
+#pragma unroll
+        for (int i = 0; i < kJoinWarps; ++i) m = fmaxf(m, sm_ml[i].x);
+#pragma unroll
+        for (int i = 0; i < kJoinWarps; ++i) {
+            if (i >= count) break;
+            const float f = sm_ml[i].x == m ? 1.f : ex2f(sm_ml[i].x - m);
+            sum += f * reinterpret_cast<const float*>(sm_o[i])[x];
+            w += f * sm_ml[i].y;
+        }
+        p.out[(long long)h.x * p.ldo + (long long)(hk * p.G + h0 + row) * D + x] = __float2bfloat16_rn(sum / w);
     }
 }
 
@@ -451,16 +536,17 @@ template <typename C>
 int launch_paged(const PagedParams& p, int ctas, cudaStream_t stream) {
     PLZ_CUDA_CHECK(cudaFuncSetAttribute(paged_attn_kernel<C>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem));
     PLZ_LAUNCH_CHAIN_BEHIND(paged_attn_kernel<C>, dim3(ctas), dim3(C::NW * 32), (size_t)C::kSmem, stream, p);
-    PLZ_LAUNCH_CHAIN_BEHIND(paged_join_kernel<C::D>, dim3(ctas), dim3(256), 0, stream, p, C::GP);
+    PLZ_LAUNCH_CHAIN_BEHIND(paged_join_kernel<C::D>, dim3(ctas, p.G < 16 ? p.G : 16), dim3(kJoinWarps * 32), 0, stream, p, C::kPart, C::NW + 2);
     return PLZ_OK;
 }
 
 }  // namespace
 
-static long long part_floats(int Hq, int Hkv, int d) { return (long long)(Hq / Hkv > 8 ? 16 : 8) * (d + 4); }
+// floats of a CTA's parts: two of the CTA's, one of each warp's
+static long long part_floats(int Hq, int Hkv, int d) { return (long long)(d == 256 ? 4 + 2 : 8 + 2) * (Hq / Hkv > 8 ? 16 : 8) * (d + 4); }
 
 long long paged_attn_ws_bytes(int Hq, int Hkv, int head_dim) {
-    return (long long)sms_of_current_device() * (2 * part_floats(Hq, Hkv, head_dim) * (long long)sizeof(float) + (long long)sizeof(int4));
+    return (long long)sms_of_current_device() * (part_floats(Hq, Hkv, head_dim) * (long long)sizeof(float) + (long long)sizeof(int4));
 }
 
 int launch_paged_attn(const PagedAttnArgs& a, void* ws, long long ws_bytes, cudaStream_t stream) {
@@ -471,16 +557,16 @@ int launch_paged_attn(const PagedAttnArgs& a, void* ws, long long ws_bytes, cuda
     p.page16 = (unsigned)(a.page_stride / 8); p.tok16 = (unsigned)(a.tok_stride / 8);
     p.table = a.table; p.ldt = a.ldt; p.lengths = a.lengths; p.out = (__nv_bfloat16*)a.out; p.ldo = a.ldo; p.bad = a.bad;
     p.parts = (float*)ws;
-    p.heads = (int4*)((char*)ws + ctas * 2 * part_floats(a.Hq, a.Hkv, a.head_dim) * (long long)sizeof(float));
+    p.heads = (int4*)((char*)ws + ctas * part_floats(a.Hq, a.Hkv, a.head_dim) * (long long)sizeof(float));
     p.B = a.B; p.width = a.width; p.page = a.page_size; p.n_pages = a.n_pages; p.Hq = a.Hq; p.Hkv = a.Hkv; p.G = a.Hq / a.Hkv;
     p.blocks = (p.G + 15) / 16; p.items = a.Hkv * p.blocks;
     p.shift = -1;
     if ((a.page_size & (a.page_size - 1)) == 0) { p.shift = 0; while ((1 << p.shift) < a.page_size) ++p.shift; }
     p.scale_log2e = a.scale * kLog2e;
     const bool wide = p.G > 8;
-    if (a.head_dim == 64) return wide ? launch_paged<Cfg<64, 16, 8, 5>>(p, ctas, stream) : launch_paged<Cfg<64, 8, 8, 6>>(p, ctas, stream);
-    if (a.head_dim == 128) return wide ? launch_paged<Cfg<128, 16, 8, 2>>(p, ctas, stream) : launch_paged<Cfg<128, 8, 8, 3>>(p, ctas, stream);
-    return wide ? launch_paged<Cfg<256, 16, 4, 2>>(p, ctas, stream) : launch_paged<Cfg<256, 8, 4, 3>>(p, ctas, stream);
+    if (a.head_dim == 64) return wide ? launch_paged<Cfg<64, 16, 32, 8, 3>>(p, ctas, stream) : launch_paged<Cfg<64, 8, 32, 8, 3>>(p, ctas, stream);
+    if (a.head_dim == 128) return wide ? launch_paged<Cfg<128, 16, 16, 8, 3>>(p, ctas, stream) : launch_paged<Cfg<128, 8, 16, 8, 3>>(p, ctas, stream);
+    return wide ? launch_paged<Cfg<256, 16, 16, 4, 3>>(p, ctas, stream) : launch_paged<Cfg<256, 8, 16, 4, 3>>(p, ctas, stream);
 }
 
 }  // namespace plz

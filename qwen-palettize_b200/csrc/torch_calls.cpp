@@ -9,6 +9,8 @@
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <cmath>
+
 #include "../../include/plz.h"
 
 namespace {
@@ -266,9 +268,147 @@ PyObject* backward_dw_soft(PyObject*, PyObject* const* a, Py_ssize_t n) {
     END_HANDLE_TH_ERRORS
 }
 
+// ---- a batch of requests of different lengths ------------------------------------------------------------------------------
+bool here(const at::Tensor& t) { return t.device().index() == c10::cuda::current_device(); }
+// int32 [n] (n < 0: any) without gaps on the current device
+const at::Tensor* numbers(PyObject* o, int64_t n = -1) {
+    const at::Tensor* t = tensor(o);
+    return t && t->scalar_type() == at::kInt && t->dim() == 1 && (n < 0 || t->size(0) == n) && t->is_contiguous() && here(*t) ? t : nullptr;
+}
+// rows of a type with unit column stride on the current device
+const at::Tensor* rows_like(PyObject* o, at::ScalarType type, int64_t n) {
+    const at::Tensor* t = tensor(o);
+    return t && t->scalar_type() == type && t->dim() == 2 && t->stride(1) == 1 && t->size(0) == n && t->size(1) <= 0x7FFFFFFF && here(*t) ? t : nullptr;
+}
+bool small(PyObject* o, int64_t& v) { return whole(o, v) && v >= 0 && v <= 0x7FFFFFFF; }
+// both pools [n_pages, page_size, cols] of one type and layout
+bool pools(PyObject* ko, PyObject* vo, int64_t cols, const at::Tensor*& k, const at::Tensor*& v) {
+    k = tensor(ko); v = tensor(vo);
+    if (!k || !v || k->scalar_type() != v->scalar_type() || k->dim() != 3 || v->dim() != 3 || k->stride(2) != 1 || k->size(2) != cols || !here(*k) || !here(*v)) return false;
+    return k->sizes() == v->sizes() && k->strides() == v->strides() && k->size(0) <= 0x7FFFFFFF && k->size(1) <= 0x7FFFFFFF;
+}
+
+// (lengths, new_tokens, table, free_pages, n_free, page_size, max_rows, row_pitch, lengths_out or None, n_free_out or None) -> (lengths, n_free, starts, slots, positions, status)
+PyObject* plan_pages(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    if (n != 10) Py_RETURN_NONE;
+    const at::Tensor *len = numbers(a[0]), *stack = numbers(a[3]), *count = numbers(a[4], 1), *tab, *len_out = nullptr, *count_out = nullptr;
+    int64_t page, rows, pitch;
+    if (!len || !stack || !count || len->size(0) > 0x7FFFFFFF || stack->size(0) > 0x7FFFFFFF || !small(a[5], page) || !small(a[6], rows) || !small(a[7], pitch)) Py_RETURN_NONE;
+    const int64_t B = len->size(0);
+    const at::Tensor* add = numbers(a[1], B);
+    if (!add || !(tab = rows_like(a[2], at::kInt, B))) Py_RETURN_NONE;
+    if ((a[8] != Py_None && !(len_out = numbers(a[8], B))) || (a[9] != Py_None && !(count_out = numbers(a[9], 1)))) Py_RETURN_NONE;
+    auto make = [&](int64_t size) { return result(*len, {size}, at::kInt); };
+    at::Tensor out[6] = {len_out ? *len_out : make(B), count_out ? *count_out : make(1), make(B + 1), make(rows), make(rows), make(B)};
+    int32_t* o[6];
+    for (int i = 0; i < 6; ++i) o[i] = (int32_t*)out[i].data_ptr();
+    const plz_page_plan_t p = {(const int32_t*)len->data_ptr(), (const int32_t*)add->data_ptr(), (int32_t*)tab->data_ptr(), tab->stride(0), (int32_t*)stack->data_ptr(),
+                               (const int32_t*)count->data_ptr(), o[0], o[1], o[2], o[3], o[4], o[5], (int32_t)B, (int32_t)tab->size(1), (int32_t)page, (int32_t)stack->size(0),
+                               (int32_t)rows, (int32_t)pitch};
+    if (!launch([&](void* s) { return plz_page_plan(&p, s); })) Py_RETURN_NONE;
+    PyObject* t = PyTuple_New(6);
+    if (!t) return nullptr;
+    for (int i = 0; i < 6; ++i) PyTuple_SET_ITEM(t, i, THPVariable_Wrap(std::move(out[i])));
+    return t;
+    END_HANDLE_TH_ERRORS
+}
+
+// (k, v, slots, k_pages, v_pages) -> True
+PyObject* write_pages(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    const at::Tensor *k, *v, *slots, *kp, *vp;
+    if (n != 5 || !(k = tensor(a[0])) || k->dim() != 2 || k->size(0) > 0x7FFFFFFF || k->stride(1) != 1 || !here(*k)) Py_RETURN_NONE;
+    const int64_t size = k->element_size(), bytes = k->size(1) * size;
+    if (!(v = rows_like(a[1], k->scalar_type(), k->size(0))) || v->size(1) != k->size(1) || !(slots = numbers(a[2], k->size(0))) || !pools(a[3], a[4], k->size(1), kp, vp) ||
+        kp->scalar_type() != k->scalar_type() || bytes > 0x7FFFFFFF) Py_RETURN_NONE;
+    const plz_page_write_t p = {k->data_ptr(), v->data_ptr(), k->stride(0) * size, v->stride(0) * size, kp->data_ptr(), vp->data_ptr(), kp->stride(0) * size, kp->stride(1) * size,
+                                (const int32_t*)slots->data_ptr(), (int32_t)k->size(0), (int32_t)bytes, (int32_t)kp->size(1), (int32_t)kp->size(0)};
+    if (!launch([&](void* s) { return plz_page_write(&p, s); })) Py_RETURN_NONE;
+    Py_RETURN_TRUE;
+    END_HANDLE_TH_ERRORS
+}
+
+// (q, k_pages, v_pages, table, lengths, heads, kv heads, head size, scale or None, out or None, bad or None) -> out
+PyObject* attention_decode_paged(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    const at::Tensor *q, *kp, *vp, *tab, *len, *out = nullptr, *bad = nullptr;
+    int64_t hq, hk, d;
+    double scale = 0.0;
+    if (n != 11 || !small(a[5], hq) || !small(a[6], hk) || !small(a[7], d) || d == 0 || hq > 0x7FFFFFFF / d || hk > 0x7FFFFFFF / d) Py_RETURN_NONE;
+    if (!(q = matrix(a[0], hq * d)) || !rows(*q) || !here(*q) || !pools(a[1], a[2], hk * d, kp, vp) || kp->scalar_type() != at::kBFloat16) Py_RETURN_NONE;
+    const int64_t B = q->size(0);
+    if (!(tab = rows_like(a[3], at::kInt, B)) || !(len = numbers(a[4], B)) || (a[8] != Py_None && !real(a[8], scale))) Py_RETURN_NONE;
+    if (a[9] != Py_None && (!(out = matrix(a[9], hq * d)) || out->size(0) != B || !here(*out))) Py_RETURN_NONE;
+    if (a[10] != Py_None && !(bad = numbers(a[10], 1))) Py_RETURN_NONE;
+    at::Tensor o = out ? *out : result(*q, {B, hq * d});
+    const int64_t bytes = plz_attn_decode_paged_ws_bytes((int32_t)hq, (int32_t)hk, (int32_t)d);
+    at::Tensor ws = result(*q, {bytes}, at::kByte);
+    const plz_attn_decode_paged_t p = {q->data_ptr(), q->stride(0), kp->data_ptr(), vp->data_ptr(), kp->stride(0), kp->stride(1), (const int32_t*)tab->data_ptr(), tab->stride(0),
+                                       (const int32_t*)len->data_ptr(), o.data_ptr(), o.stride(0), bad ? (int32_t*)bad->data_ptr() : nullptr, (int32_t)B, (int32_t)tab->size(1),
+                                       (int32_t)kp->size(1), (int32_t)kp->size(0), (int32_t)hq, (int32_t)hk, (int32_t)d, a[8] != Py_None ? (float)scale : (float)(1.0 / std::sqrt((double)d))};
+    void* const wp = ws.data_ptr();
+    if (!launch([&](void* s) { return plz_attn_decode_paged(&p, wp, bytes, s); })) Py_RETURN_NONE;
+    return THPVariable_Wrap(std::move(o));
+    END_HANDLE_TH_ERRORS
+}
+
+// a setting: None of the tensor's fields where it is a number
+bool setting(PyObject* o, int64_t n, const float*& each, float& all) {
+    double v;
+    each = nullptr; all = 0.f;
+    if (real(o, v)) { all = (float)v; return true; }
+    const at::Tensor* t = tensor(o);
+    if (!t || t->scalar_type() != at::kFloat || t->dim() != 1 || t->size(0) != n || !t->is_contiguous() || !here(*t)) return false;
+    each = (const float*)t->data_ptr();
+    return true;
+}
+
+// (logits, tokens, lengths, prompt_lengths, repetition, presence, frequency, bias_ids, bias, mask, out) -> out; tensors may be None but for the logits, settings are numbers or tensors
+PyObject* adjust_logits(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    const at::Tensor *x, *t = nullptr, *out = nullptr;
+    if (n != 11 || !(x = tensor(a[0])) || x->dim() != 2 || x->stride(1) != 1 || (x->scalar_type() != at::kFloat && x->scalar_type() != at::kBFloat16) || !here(*x)) Py_RETURN_NONE;
+    const int64_t B = x->size(0), V = x->size(1);
+    if (B > 0x7FFFFFFF || V > 0x7FFFFFFF) Py_RETURN_NONE;
+    plz_adjust_logits_t p = {};
+    p.logits = x->data_ptr(); p.ld = x->stride(0); p.rows = (int32_t)B; p.V = (int32_t)V;
+    if ((a[1] == Py_None) != (a[2] == Py_None) || (a[1] == Py_None && a[3] != Py_None) || (a[7] == Py_None) != (a[8] == Py_None)) Py_RETURN_NONE;
+    if (a[1] != Py_None) {
+        if (!(t = rows_like(a[1], at::kLong, B))) Py_RETURN_NONE;
+        p.tokens = (const int64_t*)t->data_ptr(); p.ldk = t->stride(0); p.max_tokens = (int32_t)t->size(1);
+        if (!(t = numbers(a[2], B))) Py_RETURN_NONE;
+        p.lengths = (const int32_t*)t->data_ptr();
+        if (a[3] != Py_None) {
+            if (!(t = numbers(a[3], B))) Py_RETURN_NONE;
+            p.prompt_lengths = (const int32_t*)t->data_ptr();
+        }
+    }
+    if (!setting(a[4], B, p.repetition, p.repetition_all) || !setting(a[5], B, p.presence, p.presence_all) || !setting(a[6], B, p.frequency, p.frequency_all)) Py_RETURN_NONE;
+    if (a[7] != Py_None) {
+        const at::Tensor* b;
+        if (!(t = rows_like(a[7], at::kLong, B)) || !(b = rows_like(a[8], at::kFloat, B)) || b->sizes() != t->sizes() || b->stride(0) != t->stride(0)) Py_RETURN_NONE;
+        p.bias_ids = (const int64_t*)t->data_ptr(); p.bias = (const float*)b->data_ptr(); p.ldb = t->stride(0); p.n_bias = (int32_t)t->size(1);
+    }
+    if (a[9] != Py_None) {
+        t = rows_like(a[9], at::kInt, B);
+        if (!t && !(t = rows_like(a[9], at::kInt, 1))) Py_RETURN_NONE;
+        if (t->size(1) != (V + 31) / 32) Py_RETURN_NONE;
+        p.mask = (const int32_t*)t->data_ptr(); p.ldm = t->size(0) == B ? t->stride(0) : 0;
+    }
+    if (a[10] != Py_None && (!(out = rows_like(a[10], x->scalar_type(), B)) || out->size(1) != V)) Py_RETURN_NONE;
+    at::Tensor o = out ? *out : result(*x, {B, V}, x->scalar_type());
+    p.out = o.data_ptr(); p.ldo = o.stride(0);
+    const int32_t dtype = x->scalar_type() == at::kFloat;
+    if (!launch([&](void* s) { return plz_adjust_logits(dtype, &p, s); })) Py_RETURN_NONE;
+    return THPVariable_Wrap(std::move(o));
+    END_HANDLE_TH_ERRORS
+}
+
 #define PLZ_CALL(name) {#name, (PyCFunction)(void (*)(void))name, METH_FASTCALL, nullptr}
 PyMethodDef kMethods[] = {PLZ_CALL(hard_forward), PLZ_CALL(hard_forward_smallm), PLZ_CALL(hard_forward_bias), PLZ_CALL(eval_linear), PLZ_CALL(backward_dx),
-                          PLZ_CALL(backward_dw_hard), PLZ_CALL(col_sum), PLZ_CALL(select_indices), PLZ_CALL(backward_dw_soft), {nullptr, nullptr, 0, nullptr}};
+                          PLZ_CALL(backward_dw_hard), PLZ_CALL(col_sum), PLZ_CALL(select_indices), PLZ_CALL(backward_dw_soft), PLZ_CALL(plan_pages),
+                          PLZ_CALL(write_pages), PLZ_CALL(attention_decode_paged), PLZ_CALL(adjust_logits), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_plz_torch", nullptr, -1, kMethods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

@@ -651,6 +651,9 @@ def plan_pages(lengths: torch.Tensor, new_tokens: torch.Tensor, table: torch.Ten
     the step brings, in order of the requests (row_pitch > 0: row_pitch rows for every request); a negative number ends the request and gives its pages back. table int32 [B, width] names
     the requests' pages and gets the new ones; free_pages int32 [n_pages], whose first n_free (int32 [1]) entries are free, taken from the end. A request that the free pages or `width` pages do not
     suffice for keeps what it has (status). lengths_out, n_free_out: where the new counts go, `lengths` and `n_free` themselves for a step that is captured; None: new tensors."""
+    got = P.calls().plan_pages(lengths, new_tokens, table, free_pages, n_free, page_size, max_rows, row_pitch, lengths_out, n_free_out)
+    if got is not None:
+        return PagePlan(*got)
     B = lengths.shape[0]
     _int32(lengths, (B,), "lengths"), _int32(new_tokens, (B,), "new_tokens"), _int32(n_free, (1,), "n_free"), _int32(free_pages, free_pages.shape[:1], "free_pages")
     assert table.dtype == torch.int32 and table.dim() == 2 and table.shape[0] == B and table.stride(1) == 1, "table: int32 [B, width] with unit column stride"
@@ -676,6 +679,8 @@ def _pools(k_pages: torch.Tensor, v_pages: torch.Tensor, cols: int):
 
 def write_pages(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor):
     """Rows of k and v [rows, width] into their slots of the pools [n_pages, page_size, width], any type of one size; rows with slot -1 are skipped, the others' slots differ."""
+    if P.calls().write_pages(k, v, slots, k_pages, v_pages):
+        return
     assert k.dim() == 2 and k.shape == v.shape and k.dtype == v.dtype == k_pages.dtype and k.stride(1) == v.stride(1) == 1, "k, v: rows of the pools' type, unit column stride"
     rows, W = k.shape
     _pools(k_pages, v_pages, W)
@@ -692,6 +697,9 @@ def attention_decode_paged(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torc
     """Attention of one new token per request over the request's own length of cached tokens (its own among them). q bf16 [B, n_heads * head_dim], pools bf16
     [n_pages, page_size, n_kv_heads * head_dim], table int32 [B, width], lengths int32 [B] on the device (0: zeros). Returns bf16 [B, n_heads * head_dim]. bad (int32 [1]) is set to 1
     where a page lies outside the pool (its tokens are left out) or a length outside the table."""
+    got = P.calls().attention_decode_paged(q, k_pages, v_pages, table, lengths, n_heads, n_kv_heads, head_dim, scale, out, bad)
+    if got is not None:
+        return got
     cols, B = n_heads * head_dim, q.shape[0]
     _rows(q, (B, cols), "q")
     _pools(k_pages, v_pages, n_kv_heads * head_dim)

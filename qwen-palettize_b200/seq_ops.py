@@ -274,6 +274,9 @@ def adjust_logits(logits: torch.Tensor, tokens=None, lengths=None, prompt_length
     `tokens` (int64 [rows, n], lengths int32 [rows]); x - frequency * count - presence for those that occur `count` times behind the first prompt_lengths[row] of them; the biases
     (fp32 [rows, n]) of the tokens bias_ids (int64 [rows, n], -1: nobody's); -inf where bit t % 32 of mask[row, t // 32] (int32, [rows or 1, ceil(V / 32)]) is 0. repetition, presence, frequency:
     a number or fp32 [rows]. out may be `logits`."""
+    got = P.calls().adjust_logits(logits, tokens, lengths, prompt_lengths, repetition, presence, frequency, bias_ids, bias, mask, out)
+    if got is not None:
+        return got
     assert logits.dim() == 2 and (logits.stride(1) == 1 or logits.shape[1] <= 1), "logits: [rows, V] with unit column stride"
     rows, V = logits.shape
     dtype = code(logits.dtype)
