@@ -3,14 +3,15 @@
 //   x = x > 0 ? x / r : x * r  for tokens that occur;  x - f * c - p  for those that occur c > 0 times behind the prompt;  + biases;  -inf where the mask has a 0.
 //
 // Bound by memory (a logit read and written once) from a few rows on. One CTA takes a segment of a row: it counts the row's tokens that fall into the segment in shared memory (exact and in any
-// order), and then streams the segment once, 16 bytes a thread and access. A token with a bias is marked in its count; who meets the mark walks the row's list of biases, so that
-// several biases of one token are added in the order of the list whatever the threads do.
+// order), while the segment itself is on its way to registers, 16 bytes a thread and access. A warp lists the biases that fall into the segment in their order and marks their tokens' counts; who
+// meets a mark walks that short list, so that several biases of one token are added in the order of the row's list whatever the threads do.
 #include "plz_launch.h"
 
 namespace plz {
 namespace {
 
-constexpr int kAdjThreads = 256;
+constexpr int kAdjThreads = 1024, kAdjUnits = 2;      // 16-byte units of a thread: all of a segment's logits are in registers at once
+constexpr int kAdjBiases = 4096;         // of a row at most
 constexpr uint32_t kSeen = 0x80000000u, kBiased = 0x40000000u, kCount = 0x3FFFFFFFu;
 
 struct AdjParams {
@@ -47,15 +48,14 @@ template <> struct Pack<__nv_bfloat16> {
 
 struct RowSettings { float r, p, f; };
 
-__device__ __forceinline__ float adjusted(float x, uint32_t n, int t, const RowSettings& s, const AdjParams& p, int row) {
+// ids, bias: the segment's biases in the order of the row's list
+__device__ __forceinline__ float adjusted(float x, uint32_t n, int t, const RowSettings& s, const int* ids, const float* bias, int n_bias) {
     if (n & (kSeen | kCount)) x = x > 0.f ? x / s.r : x * s.r;
     if (n & kCount) x = x - s.f * (float)(n & kCount) - s.p;
     if (n & kBiased) {
-        const long long* ids = p.bias_ids + row * p.ldb;
-        const float* b = p.bias + row * p.ldb;
         float sum = 0.f;
-        for (int i = 0; i < p.n_bias; ++i)
-            if (ids[i] == t) sum += b[i];
+        for (int i = 0; i < n_bias; ++i)
+            if (ids[i] == t) sum += bias[i];
         x += sum;
     }
     return x;
@@ -66,14 +66,39 @@ template <typename T>
 __global__ void __launch_bounds__(kAdjThreads)
 adjust_logits_kernel(const AdjParams p) {
     constexpr int N = Pack<T>::N;
-    extern __shared__ uint32_t count[];
+    extern __shared__ __align__(16) uint32_t count[];
+    __shared__ int sm_biases;
+    int* const ids = reinterpret_cast<int*>(count + p.seg + 2 * N);
+    float* const bias = reinterpret_cast<float*>(ids + p.n_bias);
     const int row = blockIdx.y, tid = threadIdx.x;
     const T* in = (const T*)p.in + row * p.ld;
     T* out = (T*)p.out + row * p.ldo;
     const int head = (int)(((16u - (uint32_t)((uintptr_t)in & 15)) & 15u) / sizeof(T));
     const int s0 = blockIdx.x ? min(p.V, head + (int)blockIdx.x * p.seg) : 0, s1 = blockIdx.x + 1 == gridDim.x ? p.V : min(p.V, head + (int)(blockIdx.x + 1) * p.seg);
+    const bool vec = (((uintptr_t)(out + head)) & 15) == 0;
+    const int v0 = blockIdx.x ? s0 : min(head, s1), v1 = vec ? v0 + (s1 - v0) / N * N : v0;      // whole 16-byte units, at most kAdjUnits a thread
+    // segment t -> count[t - s0 + pad]: the first of a unit on a 16-byte boundary
+    const int pad = (N - (v0 - s0) % N) % N;
+    if (p.lengths || p.n_bias > 0)
+        for (int i = tid; i < (pad + s1 - s0 + 3) / 4; i += kAdjThreads) reinterpret_cast<uint4*>(count)[i] = make_uint4(0u, 0u, 0u, 0u);
     pdl_launch_dependents();
     pdl_wait();
+    // the segment's logits and masks are on their way while its tokens are counted
+    const int* mask = p.mask ? p.mask + row * p.ldm : nullptr;
+    const int words = (p.V + 31) >> 5;
+    uint4 raw[kAdjUnits];
+    uint32_t bits[kAdjUnits];
+#pragma unroll
+    for (int k = 0; k < kAdjUnits; ++k) {
+        const int i = v0 + (k * kAdjThreads + tid) * N;
+        bits[k] = 0xFFFFFFFFu;
+        if (i >= v1) continue;
+        raw[k] = *reinterpret_cast<const uint4*>(in + i);
+        if (mask) {
+            const int w = i >> 5;
+            bits[k] = __funnelshift_r((uint32_t)mask[w], w + 1 < words ? (uint32_t)mask[w + 1] : 0u, i & 31);
+        }
+    }
     RowSettings s;
     s.r = p.repetition ? p.repetition[row] : p.repetition_all;
     s.p = p.presence ? p.presence[row] : p.presence_all;
@@ -81,42 +106,72 @@ adjust_logits_kernel(const AdjParams p) {
     const int n_tok = p.lengths ? min(max(p.lengths[row], 0), p.max_tokens) : 0, n_prompt = p.prompt_lengths ? max(p.prompt_lengths[row], 0) : 0;
     const bool marks = n_tok > 0 || p.n_bias > 0;
     if (marks) {
-        for (int i = tid; i < s1 - s0; i += kAdjThreads) count[i] = 0;
         __syncthreads();
         const long long* tok = p.tokens + row * p.ldk;
-        for (int i = tid; i < n_tok; i += kAdjThreads) {
-            const long long t = tok[i] - s0;
-            if (t < 0 || t >= s1 - s0) continue;
-            if (i < n_prompt) atomicOr(count + t, kSeen); else atomicAdd(count + t, 1u);
+        constexpr int U = 8;                   // tokens of a thread that are asked for together
+        for (int i0 = tid; i0 < n_tok; i0 += kAdjThreads * U) {
+            long long t[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) t[u] = i0 + u * kAdjThreads < n_tok ? tok[i0 + u * kAdjThreads] - s0 : -1;
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                if (t[u] < 0 || t[u] >= s1 - s0) continue;
+                if (i0 + u * kAdjThreads < n_prompt) atomicOr(count + pad + t[u], kSeen); else atomicAdd(count + pad + t[u], 1u);
+            }
         }
-        const long long* ids = p.bias_ids + row * p.ldb;
-        for (int i = tid; i < p.n_bias; i += kAdjThreads) {
-            const long long t = ids[i] - s0;
-            if (t >= 0 && t < s1 - s0) atomicOr(count + t, kBiased);
+        if (p.n_bias > 0 && tid >= kAdjThreads - 32) {
+            // one warp keeps what falls into the segment, in its order
+            const int lane = tid & 31;
+            const long long* from = p.bias_ids + row * p.ldb;
+            const float* value = p.bias + row * p.ldb;
+            int n = 0;
+            constexpr int U = 4;
+            for (int i0 = lane; i0 - lane < p.n_bias; i0 += 32 * U) {
+                long long t[U];
+                float v[U];
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    const bool in = i0 + 32 * u < p.n_bias;
+                    t[u] = in ? from[i0 + 32 * u] - s0 : -1;
+                    v[u] = in ? value[i0 + 32 * u] : 0.f;
+                }
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    const bool in = t[u] >= 0 && t[u] < s1 - s0;
+                    const uint32_t all = __ballot_sync(0xFFFFFFFFu, in);
+                    if (in) {
+                        const int at = n + __popc(all & ((1u << lane) - 1u));
+                        ids[at] = s0 + (int)t[u];
+                        bias[at] = v[u];
+                        atomicOr(count + pad + t[u], kBiased);
+                    }
+                    n += __popc(all);
+                }
+            }
+            if (lane == 0) sm_biases = n;
         }
         __syncthreads();
     }
-    const int* mask = p.mask ? p.mask + row * p.ldm : nullptr;
-    const int words = (p.V + 31) >> 5;
-    const bool vec = (((uintptr_t)(out + head)) & 15) == 0;
-    const int v0 = blockIdx.x ? s0 : min(head, s1), v1 = vec ? v0 + (s1 - v0) / N * N : v0;
-    for (int i = v0 + tid * N; i < v1; i += kAdjThreads * N) {
+    const int n_bias = p.n_bias > 0 ? sm_biases : 0;
+#pragma unroll
+    for (int k = 0; k < kAdjUnits; ++k) {
+        const int i = v0 + (k * kAdjThreads + tid) * N;
+        if (i >= v1) continue;
         float x[N];
-        Pack<T>::unpack(*reinterpret_cast<const uint4*>(in + i), x);
+        Pack<T>::unpack(raw[k], x);
         if (marks) {
 #pragma unroll
-            for (int e = 0; e < N; ++e) {
-                const uint32_t n = count[i - s0 + e];
-                if (n) x[e] = adjusted(x[e], n, i + e, s, p, row);
+            for (int q = 0; q < N / 4; ++q) {
+                const uint4 n4 = reinterpret_cast<const uint4*>(count)[(pad + i - s0) / 4 + q];
+                const uint32_t n[4] = {n4.x, n4.y, n4.z, n4.w};
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (n[e]) x[4 * q + e] = adjusted(x[4 * q + e], n[e], i + 4 * q + e, s, ids, bias, n_bias);
             }
         }
-        if (mask) {
-            const int w = i >> 5;
-            const uint32_t lo = mask[w], hi = w + 1 < words ? mask[w + 1] : 0u, bits = __funnelshift_r(lo, hi, i & 31);
 #pragma unroll
-            for (int e = 0; e < N; ++e)
-                if (!((bits >> e) & 1u)) x[e] = -INFINITY;
-        }
+        for (int e = 0; e < N; ++e)
+            if (!((bits[k] >> e) & 1u)) x[e] = -INFINITY;
         *reinterpret_cast<uint4*>(out + i) = Pack<T>::pack(x);
     }
     // what is not whole 16 bytes: in front of the first boundary, behind the last, or the segment where in and out lie differently
@@ -125,8 +180,8 @@ adjust_logits_kernel(const AdjParams p) {
         const int i = j < front ? s0 + j : v1 + j - front;
         float x = Pack<T>::get(in[i]);
         if (marks) {
-            const uint32_t n = count[i - s0];
-            if (n) x = adjusted(x, n, i, s, p, row);
+            const uint32_t n = count[pad + i - s0];
+            if (n) x = adjusted(x, n, i, s, ids, bias, n_bias);
         }
         if (mask && !((mask[i >> 5] >> (i & 31)) & 1)) x = -INFINITY;
         out[i] = Pack<T>::put(x);
@@ -136,9 +191,20 @@ adjust_logits_kernel(const AdjParams p) {
 template <typename T>
 int launch_adjust(const AdjustLogitsArgs& a, cudaStream_t stream) {
     AdjParams p = {a.logits, a.ld, a.out, a.ldo, (const long long*)a.tokens, a.ldk, a.lengths, a.prompt_lengths, a.repetition, a.presence, a.frequency, (const long long*)a.bias_ids, a.bias,
-                   a.ldb, a.mask, a.ldm, a.repetition_all, a.presence_all, a.frequency_all, a.V, a.max_tokens, a.n_bias, 8192};
-    const int segs = (a.V + p.seg - 1) / p.seg;
-    PLZ_LAUNCH_CHAIN_BEHIND(adjust_logits_kernel<T>, dim3(segs, a.rows), dim3(kAdjThreads), (size_t)(p.seg + Pack<T>::N) * sizeof(uint32_t), stream, p);
+                   a.ldb, a.mask, a.ldm, a.repetition_all, a.presence_all, a.frequency_all, a.V, a.max_tokens, a.n_bias, 0};
+    // the largest segment, whose tokens are read by the fewest CTAs, that still gives every SM one
+    const int sms = sms_of_current_device();
+    p.seg = kAdjThreads * kAdjUnits * Pack<T>::N;
+    while (p.seg > 2048 && (long long)a.rows * ((a.V + p.seg - 1) / p.seg) < sms) p.seg /= 2;
+    const size_t smem = (size_t)(p.seg + 2 * Pack<T>::N + 2 * a.n_bias) * sizeof(uint32_t);
+    static bool once[64] = {};
+    int dev = 0;
+    PLZ_CUDA_CHECK(cudaGetDevice(&dev));
+    if (!once[dev & 63]) {
+        PLZ_CUDA_CHECK(cudaFuncSetAttribute(adjust_logits_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, ((kAdjThreads * kAdjUnits + 2) * Pack<T>::N + 2 * kAdjBiases) * (int)sizeof(uint32_t)));
+        once[dev & 63] = true;
+    }
+    PLZ_LAUNCH_CHAIN_BEHIND(adjust_logits_kernel<T>, dim3((a.V + p.seg - 1) / p.seg, a.rows), dim3(kAdjThreads), smem, stream, p);
     return PLZ_OK;
 }
 

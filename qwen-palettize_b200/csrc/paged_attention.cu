@@ -534,7 +534,10 @@ paged_join_kernel(const PagedParams p, int part, int per_cta) {
 
 template <typename C>
 int launch_paged(const PagedParams& p, int ctas, cudaStream_t stream) {
-    PLZ_CUDA_CHECK(cudaFuncSetAttribute(paged_attn_kernel<C>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem));
+    static bool once[64] = {};
+    int dev = 0;
+    PLZ_CUDA_CHECK(cudaGetDevice(&dev));
+    if (!once[dev & 63]) { PLZ_CUDA_CHECK(cudaFuncSetAttribute(paged_attn_kernel<C>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem)); once[dev & 63] = true; }
     PLZ_LAUNCH_CHAIN_BEHIND(paged_attn_kernel<C>, dim3(ctas), dim3(C::NW * 32), (size_t)C::kSmem, stream, p);
     PLZ_LAUNCH_CHAIN_BEHIND(paged_join_kernel<C::D>, dim3(ctas, p.G < 16 ? p.G : 16), dim3(kJoinWarps * 32), 0, stream, p, C::kPart, C::NW + 2);
     return PLZ_OK;
