@@ -92,11 +92,15 @@ struct Cfg {
     static constexpr int D = D_, GP = GP_, TOK = TOK_, NW = NW_, NST = NST_;
     static constexpr int kTile = TOK * D * 2;                       // bytes of a step's keys, or values
     static constexpr int kStage = 2 * kTile;
+    static constexpr int kFree = 227 * 1024 - NW * NST * kStage - (NW * 32 * 8 + NW * (2 * 16 + 2 * NST * 16 + NST * TOK * 4 + NST * 4 + 8)) - 256;    // shared memory without the rings and the rest
     static constexpr int kPitch = D + 4;                            // floats between rows of a part: D sums, maximum, sum of weights
     static constexpr int kPart = GP * kPitch;                       // floats
-    static constexpr int kWarp = NST * kStage;                      // a warp's shared memory: its ring; the part that it ends with takes the ring's place
+    static constexpr int kRing = NST * kStage;
+    // the part that a warp ends with takes the place of its ring; the one that it began with lies behind the ring, as far as it has rows that fit
+    static constexpr int kRows = kFree / NW / (kPitch * 4) < GP ? kFree / NW / (kPitch * 4) : GP;
+    static constexpr int kWarp = kRing + kRows * kPitch * 4;        // a warp's shared memory
     static constexpr int kSmem = NW * kWarp;
-    static_assert(kPart * 4 <= kWarp, "the last part lies in the ring");
+    static_assert(kPart * 4 <= kRing, "the last part lies in the ring");
 };
 struct PartMeta { int b, item, flags, rest; };      // flags 1: valid, 2: holds the head's first step, 4: holds its last; rest: steps behind it
 
@@ -168,6 +172,7 @@ paged_attn_kernel(const PagedParams p) {
         }
     }
 
+    auto first_part = [&](int w) { return p.G <= C::kRows ? reinterpret_cast<float*>(smem + w * C::kWarp + C::kRing) : p.parts + ((size_t)cta * (2 + NW) + 2 + w) * C::kPart; };
     uint8_t* const mine_smem = smem + warp * C::kWarp;
     const uint32_t ring = smem_u32(mine_smem);
     if (eye.left > 0) {
@@ -364,10 +369,11 @@ paged_attn_kernel(const PagedParams p) {
                         for (int n = 0; n < D / 8; ++n) *reinterpret_cast<uint32_t*>(o + n * 8) = pack_bf16x2(acc[n][2 * r] * inv, acc[n][2 * r + 1] * inv);
                     }
                 } else {
-                    // the part that a warp ends with goes to the place of its ring, into which nothing comes any more, the one that it began with, while the ring is at work, to the workspace
-                    float* const part = over ? reinterpret_cast<float*>(mine_smem) : p.parts + ((size_t)cta * (2 + NW) + 2 + warp) * C::kPart;
+                    // the part that a warp ends with goes to the place of its ring, into which nothing comes any more, the one that it began with, while the ring is at work, behind it
+                    float* const part = over ? reinterpret_cast<float*>(mine_smem) : first_part(warp);
 #pragma unroll
                     for (int r = 0; r < NR; ++r) {
+                        if (g + 8 * r >= heads) continue;
                         float* row = part + (g + 8 * r) * C::kPitch;
 #pragma unroll
                         for (int n = 0; n < D / 8; ++n) *reinterpret_cast<float2*>(row + n * 8 + c2) = make_float2(acc[n][2 * r], acc[n][2 * r + 1]);
@@ -384,9 +390,7 @@ paged_attn_kernel(const PagedParams p) {
     __syncthreads();
 
     // ---- the parts of this CTA, in order: those of one head follow one another. A warp takes a head and one of its rows at a time.
-    auto part_at = [&](int i) -> const float* {
-        return i & 1 ? reinterpret_cast<const float*>(smem + (i >> 1) * C::kWarp) : p.parts + ((size_t)cta * (2 + NW) + 2 + (i >> 1)) * C::kPart;
-    };
+    auto part_at = [&](int i) -> const float* { return i & 1 ? reinterpret_cast<const float*>(smem + (i >> 1) * C::kWarp) : first_part(i >> 1); };
     const PartMeta own = lane < 2 * NW ? sm_meta[lane >> 1][lane & 1] : PartMeta{0, 0, 0, 0};
     const uint32_t valid = __ballot_sync(0xFFFFFFFFu, own.flags & 1), starts = __ballot_sync(0xFFFFFFFFu, (own.flags & 3) == 3) | (valid & -valid);
     const uint32_t ends = __ballot_sync(0xFFFFFFFFu, (own.flags & 5) == 5), begun = __ballot_sync(0xFFFFFFFFu, (own.flags & 3) == 3);
@@ -422,24 +426,25 @@ paged_attn_kernel(const PagedParams p) {
 #pragma unroll
             for (int n = 0; n < (D + 127) / 128; ++n) {
                 const int d = n * 128 + lane * 4;
-                // All parts are asked for ahead of the sum, without branches: what is no part of the run is whatever lies there, and left out. Only few heads have one in the workspace.
-                float4 v[2 * NW];
-                const int at = row * C::kPitch + (d < D ? d : 0);
-#pragma unroll
-                for (int j = 1; j < 2 * NW; j += 2) v[j] = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(smem + (j >> 1) * C::kWarp) + at);
-                if (run & 0x55555555u) {
-#pragma unroll
-                    for (int j = 0; j < 2 * NW; j += 2) v[j] = *reinterpret_cast<const float4*>(p.parts + ((size_t)cta * (2 + NW) + 2 + (j >> 1)) * C::kPart + at);
-                } else {
-#pragma unroll
-                    for (int j = 0; j < 2 * NW; j += 2) v[j] = make_float4(0.f, 0.f, 0.f, 0.f);
-                }
                 float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+                const int at = row * C::kPitch + (d < D ? d : 0);
+                for (uint32_t left = run; left;) {
+                    // four at a time; past the last one that one again, without weight
+                    int j[4];
+                    float fj[4];
+                    float4 v[4];
 #pragma unroll
-                for (int j = 0; j < 2 * NW; ++j) {
-                    const float fj = __shfl_sync(0xFFFFFFFFu, f, j);
-                    const bool in = (run >> j) & 1u;
-                    o.x += in ? fj * v[j].x : 0.f; o.y += in ? fj * v[j].y : 0.f; o.z += in ? fj * v[j].z : 0.f; o.w += in ? fj * v[j].w : 0.f;
+                    for (int k = 0; k < 4; ++k) {
+                        j[k] = left ? __ffs(left) - 1 : j[k > 0 ? k - 1 : 0];
+                        fj[k] = left ? 1.f : 0.f;
+                        left &= left - 1u;
+                        v[k] = *reinterpret_cast<const float4*>(part_at(j[k]) + at);
+                    }
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        fj[k] *= __shfl_sync(0xFFFFFFFFu, f, j[k]);
+                        o.x += fj[k] * v[k].x; o.y += fj[k] * v[k].y; o.z += fj[k] * v[k].z; o.w += fj[k] * v[k].w;
+                    }
                 }
                 if (d >= D) continue;
                 if (first && last) {

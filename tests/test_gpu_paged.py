@@ -206,6 +206,25 @@ def test_attention_lengths(page, lengths):
     check_status()
 
 
+@pytest.mark.parametrize("hq,hk,d,page,B,T", [(32, 8, 128, 16, 70, 1500), (16, 16, 64, 64, 200, 700), (8, 2, 256, 32, 40, 3000), (40, 2, 128, 16, 60, 5000), (4, 1, 128, 16, 1, 600000), (9, 3, 64, 128, 2000, 300)])
+def test_attention_with_many_steps(hq, hk, d, page, B, T):
+    """Enough work for it to be taken as it comes: right, and the same bits whoever takes it."""
+    import plz_ops as ops
+    g = torch.Generator().manual_seed(B)
+    lengths = torch.randint(T // 2, T + 1, (B,), generator=g).tolist()
+    lengths[B // 3] = 0 if B > 1 else lengths[0]
+    width = -(-T // page)
+    dev = torch.Generator(device="cuda").manual_seed(B)
+    table = torch.randperm(B * width, generator=dev, device="cuda").to(I32).view(B, width)
+    kp, vp = (torch.randn(B * width, page, hk * d, generator=dev, device="cuda").bfloat16() for _ in range(2))
+    q = torch.randn(B, hq * d, generator=dev, device="cuda").bfloat16()
+    a = (q, kp, vp, table, _dev(lengths))
+    got = [ops.attention_decode_paged(*a, hq, hk, d) for _ in range(4)]
+    check_status()
+    _close(got[0], *ref.attention(*a, hq, hk, d))
+    assert all(torch.equal(got[0], x) for x in got[1:])
+
+
 @pytest.mark.parametrize("scale", [1.0, 0.02, -0.3, 0.0])
 def test_attention_scale_and_layouts(scale):
     """Pitched q, out and table, pools that are slices of a larger one."""
