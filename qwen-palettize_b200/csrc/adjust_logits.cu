@@ -2,15 +2,19 @@
 //
 //   x = x > 0 ? x / r : x * r  for tokens that occur;  x - f * c - p  for those that occur c > 0 times behind the prompt;  + biases;  -inf where the mask has a 0.
 //
-// Bound by memory (a logit read and written once) from a few rows on. One CTA takes a segment of a row: it counts the row's tokens that fall into the segment in shared memory (exact and in any
-// order), while the segment itself is on its way to registers, 16 bytes a thread and access. A warp lists the biases that fall into the segment in their order and marks their tokens' counts; who
-// meets a mark walks that short list, so that several biases of one token are added in the order of the row's list whatever the threads do.
+// Bound by memory (a logit read and written once) from a few rows on. Few tokens of a vocabulary are touched, so the penalties and biases stay out of the stream of all logits: with them in it,
+// 50 instructions a logit, 64 rows of 151936 took 30 us, bound by issue.
+//   A CTA takes a segment of a row, copies it through the mask, 16 bytes a thread and access, and counts the row's tokens that fall into it in shared memory (whole numbers, exact in any order);
+//   reading all tokens in every CTA costs less than a cluster that reads them once and counts in its distributed shared memory (8 rows with 30000 tokens 18 us, 64 rows 38 us: its CTAs wait for one
+//   another, and its atomics are slow). One warp lists the biases of the segment's tokens in their order and marks the tokens' counts; several biases of one token are added in the order of
+//   the row's list whatever the threads do. Then the marked logits are computed and stored over the copy.
 #include "plz_launch.h"
 
 namespace plz {
 namespace {
 
-constexpr int kAdjThreads = 1024, kAdjUnits = 2;      // 16-byte units of a thread: all of a segment's logits are in registers at once
+constexpr int kAdjThreads = 512, kAdjUnits = 2, kAdjTokens = 8, kAdjMarks = 4;      // 16-byte units, tokens, marked logits of a thread that are on their way at once
+constexpr int kAdjLargest = 20480;                    // logits of a CTA at most (80 KB of counts, two CTAs per SM)
 constexpr int kAdjBiases = 4096;         // of a row at most
 constexpr uint32_t kSeen = 0x80000000u, kBiased = 0x40000000u, kCount = 0x3FFFFFFFu;
 
@@ -31,160 +35,190 @@ template <> struct Pack<float> {
     static constexpr int N = 4;
     __device__ __forceinline__ static float get(float v) { return v; }
     __device__ __forceinline__ static float put(float v) { return v; }
-    __device__ __forceinline__ static void unpack(const uint4& v, float (&f)[4]) { f[0] = __uint_as_float(v.x); f[1] = __uint_as_float(v.y); f[2] = __uint_as_float(v.z); f[3] = __uint_as_float(v.w); }
-    __device__ __forceinline__ static uint4 pack(const float (&f)[4]) { return make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3])); }
+    // -inf where the bit is 0
+    __device__ __forceinline__ static uint4 masked(const uint4& v, uint32_t bits) {
+        return make_uint4(bits & 1u ? v.x : 0xFF800000u, bits & 2u ? v.y : 0xFF800000u, bits & 4u ? v.z : 0xFF800000u, bits & 8u ? v.w : 0xFF800000u);
+    }
 };
 template <> struct Pack<__nv_bfloat16> {
     static constexpr int N = 8;
     __device__ __forceinline__ static float get(__nv_bfloat16 v) { return __bfloat162float(v); }
     __device__ __forceinline__ static __nv_bfloat16 put(float v) { return __float2bfloat16_rn(v); }
-    __device__ __forceinline__ static void unpack(const uint4& v, float (&f)[8]) {
-        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) { f[2 * i] = __uint_as_float(w[i] << 16); f[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u); }
-    }
-    __device__ __forceinline__ static uint4 pack(const float (&f)[8]) { return make_uint4(pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]), pack_bf16x2(f[4], f[5]), pack_bf16x2(f[6], f[7])); }
+    __device__ __forceinline__ static uint32_t two(uint32_t w, uint32_t bits) { return (bits & 1u ? w & 0xFFFFu : 0xFF80u) | (bits & 2u ? w & 0xFFFF0000u : 0xFF800000u); }
+    __device__ __forceinline__ static uint4 masked(const uint4& v, uint32_t bits) { return make_uint4(two(v.x, bits), two(v.y, bits >> 2), two(v.z, bits >> 4), two(v.w, bits >> 6)); }
 };
 
-struct RowSettings { float r, p, f; };
+struct RowSettings { float r, inv, p, f; };      // inv = 1 / r: x * inv is within 2^-23 of x / r
 
-// ids, bias: the segment's biases in the order of the row's list
-__device__ __forceinline__ float adjusted(float x, uint32_t n, int t, const RowSettings& s, const int* ids, const float* bias, int n_bias) {
-    if (n & (kSeen | kCount)) x = x > 0.f ? x / s.r : x * s.r;
-    if (n & kCount) x = x - s.f * (float)(n & kCount) - s.p;
-    if (n & kBiased) {
-        float sum = 0.f;
-        for (int i = 0; i < n_bias; ++i)
-            if (ids[i] == t) sum += bias[i];
-        x += sum;
-    }
-    return x;
+__device__ __forceinline__ float penalized(float x, uint32_t n, const RowSettings& s) {
+    const uint32_t c = n & kCount;
+    if (n & (kSeen | kCount)) x *= x > 0.f ? s.inv : s.r;
+    return c ? x - s.f * (float)c - s.p : x;
 }
 
-// `seg` logits from the first 16-byte boundary of the row on; the few in front of it belong to the first segment
+// CTA c has the `seg` logits from c * seg behind the row's first 16-byte boundary on, the first CTA the few in front of it too. A CTA's logits have numbers of their own, `own`: logit t
+// is N + t - v0, so that a unit's counts begin on a 16-byte boundary.
 template <typename T>
-__global__ void __launch_bounds__(kAdjThreads)
+__global__ void __launch_bounds__(kAdjThreads, 2)
 adjust_logits_kernel(const AdjParams p) {
     constexpr int N = Pack<T>::N;
-    extern __shared__ __align__(16) uint32_t count[];
+    extern __shared__ __align__(16) uint32_t count[];                       // [N + seg]
     __shared__ int sm_biases;
-    int* const ids = reinterpret_cast<int*>(count + p.seg + 2 * N);
+    int* const ids = reinterpret_cast<int*>(count + N + p.seg);            // biases of this CTA's tokens
     float* const bias = reinterpret_cast<float*>(ids + p.n_bias);
-    const int row = blockIdx.y, tid = threadIdx.x;
+    const int row = blockIdx.y, tid = threadIdx.x, lane = tid & 31;
     const T* in = (const T*)p.in + row * p.ld;
     T* out = (T*)p.out + row * p.ldo;
-    const int head = (int)(((16u - (uint32_t)((uintptr_t)in & 15)) & 15u) / sizeof(T));
-    const int s0 = blockIdx.x ? min(p.V, head + (int)blockIdx.x * p.seg) : 0, s1 = blockIdx.x + 1 == gridDim.x ? p.V : min(p.V, head + (int)(blockIdx.x + 1) * p.seg);
-    const bool vec = (((uintptr_t)(out + head)) & 15) == 0;
-    const int v0 = blockIdx.x ? s0 : min(head, s1), v1 = vec ? v0 + (s1 - v0) / N * N : v0;      // whole 16-byte units, at most kAdjUnits a thread
-    // segment t -> count[t - s0 + pad]: the first of a unit on a 16-byte boundary
-    const int pad = (N - (v0 - s0) % N) % N;
-    if (p.lengths || p.n_bias > 0)
-        for (int i = tid; i < (pad + s1 - s0 + 3) / 4; i += kAdjThreads) reinterpret_cast<uint4*>(count)[i] = make_uint4(0u, 0u, 0u, 0u);
+    const int head = min((int)(((16u - (uint32_t)((uintptr_t)in & 15)) & 15u) / sizeof(T)), p.V);
+    const int v0 = min(head + (int)blockIdx.x * p.seg, p.V), s0 = blockIdx.x ? v0 : 0, s1 = blockIdx.x + 1 == gridDim.x ? p.V : min(v0 + p.seg, p.V);
+    const bool vec = (((uintptr_t)(out + head)) & 15) == 0, marks = (p.lengths && p.max_tokens > 0) || p.n_bias > 0;
+    if (marks) {
+        for (int i = tid; i < (N + p.seg) / 4; i += kAdjThreads) reinterpret_cast<uint4*>(count)[i] = make_uint4(0u, 0u, 0u, 0u);
+        if (tid == 0) sm_biases = 0;
+    }
     pdl_launch_dependents();
     pdl_wait();
-    // the segment's logits and masks are on their way while its tokens are counted
     const int* mask = p.mask ? p.mask + row * p.ldm : nullptr;
     const int words = (p.V + 31) >> 5;
-    uint4 raw[kAdjUnits];
-    uint32_t bits[kAdjUnits];
-#pragma unroll
-    for (int k = 0; k < kAdjUnits; ++k) {
-        const int i = v0 + (k * kAdjThreads + tid) * N;
-        bits[k] = 0xFFFFFFFFu;
-        if (i >= v1) continue;
-        raw[k] = *reinterpret_cast<const uint4*>(in + i);
+    // a unit of 16 bytes and its mask words, shifted when they are needed
+    struct Unit { uint4 raw; uint32_t lo, hi; };
+    auto load = [&](int t, Unit& u) {
+        u.lo = u.hi = 0xFFFFFFFFu;
+        if (!vec || t + N > s1) return;
+        u.raw = *reinterpret_cast<const uint4*>(in + t);
         if (mask) {
-            const int w = i >> 5;
-            bits[k] = __funnelshift_r((uint32_t)mask[w], w + 1 < words ? (uint32_t)mask[w + 1] : 0u, i & 31);
+            const int w = t >> 5;
+            u.lo = mask[w];
+            u.hi = mask[min(w + 1, words - 1)];
         }
-    }
-    RowSettings s;
-    s.r = p.repetition ? p.repetition[row] : p.repetition_all;
-    s.p = p.presence ? p.presence[row] : p.presence_all;
-    s.f = p.frequency ? p.frequency[row] : p.frequency_all;
-    const int n_tok = p.lengths ? min(max(p.lengths[row], 0), p.max_tokens) : 0, n_prompt = p.prompt_lengths ? max(p.prompt_lengths[row], 0) : 0;
-    const bool marks = n_tok > 0 || p.n_bias > 0;
-    if (marks) {
-        __syncthreads();
-        const long long* tok = p.tokens + row * p.ldk;
-        constexpr int U = 8;                   // tokens of a thread that are asked for together
-        for (int i0 = tid; i0 < n_tok; i0 += kAdjThreads * U) {
-            long long t[U];
+    };
+    Unit unit[kAdjUnits];                      // the first ones are on their way while tokens are counted
 #pragma unroll
-            for (int u = 0; u < U; ++u) t[u] = i0 + u * kAdjThreads < n_tok ? tok[i0 + u * kAdjThreads] - s0 : -1;
+    for (int k = 0; k < kAdjUnits; ++k) load(v0 + (k * kAdjThreads + tid) * N, unit[k]);
+    if (marks) {
+        const int n_tok = p.lengths ? min(max(p.lengths[row], 0), p.max_tokens) : 0, n_prompt = p.prompt_lengths ? max(p.prompt_lengths[row], 0) : 0;
+        const long long* tok = p.tokens + row * p.ldk;
+        constexpr int U = kAdjTokens;          // tokens of a thread that are asked for together
+        long long t[U];
+        auto fetch = [&](int i0) {
+#pragma unroll
+            for (int u = 0; u < U; ++u) t[u] = i0 + u * kAdjThreads < n_tok ? tok[i0 + u * kAdjThreads] : -1;
+        };
+        int i0 = tid;
+        fetch(i0);
+        constexpr int UB = 4;
+        const bool lists = p.n_bias > 0 && tid >= kAdjThreads - 32;
+        long long id[UB];
+        float v[UB];
+        auto fetch_biases = [&](int j0) {
+#pragma unroll
+            for (int u = 0; u < UB; ++u) {
+                const bool more = j0 + 32 * u < p.n_bias;
+                id[u] = more ? p.bias_ids[row * p.ldb + j0 + 32 * u] : -1;
+                v[u] = more ? p.bias[row * p.ldb + j0 + 32 * u] : 0.f;
+            }
+        };
+        if (lists) fetch_biases(lane);
+        __syncthreads();                       // all counts are 0
+        for (; i0 < n_tok; i0 += kAdjThreads * U) {
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                if (t[u] < 0 || t[u] >= s1 - s0) continue;
-                if (i0 + u * kAdjThreads < n_prompt) atomicOr(count + pad + t[u], kSeen); else atomicAdd(count + pad + t[u], 1u);
+                if (t[u] < s0 || t[u] >= s1) continue;
+                uint32_t* const where = count + N + (int)t[u] - v0;
+                if (i0 + u * kAdjThreads < n_prompt) atomicOr(where, kSeen); else atomicAdd(where, 1u);
             }
+            fetch(i0 + kAdjThreads * U);
         }
-        if (p.n_bias > 0 && tid >= kAdjThreads - 32) {
-            // one warp keeps what falls into the segment, in its order
-            const int lane = tid & 31;
-            const long long* from = p.bias_ids + row * p.ldb;
-            const float* value = p.bias + row * p.ldb;
+        if (lists) {
+            // one warp keeps what belongs to this CTA, in its order
             int n = 0;
-            constexpr int U = 4;
-            for (int i0 = lane; i0 - lane < p.n_bias; i0 += 32 * U) {
-                long long t[U];
-                float v[U];
+            for (int j0 = lane; j0 - lane < p.n_bias; j0 += 32 * UB) {
 #pragma unroll
-                for (int u = 0; u < U; ++u) {
-                    const bool in = i0 + 32 * u < p.n_bias;
-                    t[u] = in ? from[i0 + 32 * u] - s0 : -1;
-                    v[u] = in ? value[i0 + 32 * u] : 0.f;
-                }
-#pragma unroll
-                for (int u = 0; u < U; ++u) {
-                    const bool in = t[u] >= 0 && t[u] < s1 - s0;
-                    const uint32_t all = __ballot_sync(0xFFFFFFFFu, in);
-                    if (in) {
+                for (int u = 0; u < UB; ++u) {
+                    const bool mine = id[u] >= s0 && id[u] < s1;
+                    const int own = N + (int)id[u] - v0;
+                    const uint32_t all = __ballot_sync(0xFFFFFFFFu, mine);
+                    if (mine) {
                         const int at = n + __popc(all & ((1u << lane) - 1u));
-                        ids[at] = s0 + (int)t[u];
+                        ids[at] = own;
                         bias[at] = v[u];
-                        atomicOr(count + pad + t[u], kBiased);
+                        atomicOr(count + own, kBiased);
                     }
                     n += __popc(all);
                 }
+                fetch_biases(j0 + 32 * UB);
             }
             if (lane == 0) sm_biases = n;
         }
-        __syncthreads();
     }
-    const int n_bias = p.n_bias > 0 ? sm_biases : 0;
+    // all logits, kAdjUnits units of a thread at a time
+    for (int t0 = v0; t0 < s1; t0 += kAdjUnits * kAdjThreads * N) {
+        if (t0 > v0) {
 #pragma unroll
-    for (int k = 0; k < kAdjUnits; ++k) {
-        const int i = v0 + (k * kAdjThreads + tid) * N;
-        if (i >= v1) continue;
-        float x[N];
-        Pack<T>::unpack(raw[k], x);
-        if (marks) {
+            for (int k = 0; k < kAdjUnits; ++k) load(t0 + (k * kAdjThreads + tid) * N, unit[k]);
+        }
 #pragma unroll
-            for (int q = 0; q < N / 4; ++q) {
-                const uint4 n4 = reinterpret_cast<const uint4*>(count)[(pad + i - s0) / 4 + q];
-                const uint32_t n[4] = {n4.x, n4.y, n4.z, n4.w};
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    if (n[e]) x[4 * q + e] = adjusted(x[4 * q + e], n[e], i + 4 * q + e, s, ids, bias, n_bias);
+        for (int k = 0; k < kAdjUnits; ++k) {
+            const int t = t0 + (k * kAdjThreads + tid) * N;
+            if (t >= s1) continue;
+            if (vec && t + N <= s1) {
+                if (mask) unit[k].raw = Pack<T>::masked(unit[k].raw, __funnelshift_r(unit[k].lo, unit[k].hi, t & 31));
+                *reinterpret_cast<uint4*>(out + t) = unit[k].raw;
+            } else {
+                // the row's end, or in and out lie differently
+                for (int e = 0; e < N && t + e < s1; ++e) out[t + e] = !mask || ((mask[(t + e) >> 5] >> ((t + e) & 31)) & 1) ? in[t + e] : Pack<T>::put(-INFINITY);
             }
         }
-#pragma unroll
-        for (int e = 0; e < N; ++e)
-            if (!((bits[k] >> e) & 1u)) x[e] = -INFINITY;
-        *reinterpret_cast<uint4*>(out + i) = Pack<T>::pack(x);
     }
-    // what is not whole 16 bytes: in front of the first boundary, behind the last, or the segment where in and out lie differently
-    const int front = v0 - s0, rest = front + s1 - v1;
-    for (int j = tid; j < rest; j += kAdjThreads) {
-        const int i = j < front ? s0 + j : v1 + j - front;
-        float x = Pack<T>::get(in[i]);
-        if (marks) {
-            const uint32_t n = count[pad + i - s0];
-            if (n) x = adjusted(x, n, i, s, ids, bias, n_bias);
+    if (tid < v0 - s0) out[tid] = !mask || ((mask[0] >> tid) & 1) ? in[tid] : Pack<T>::put(-INFINITY);
+    if (!marks) return;
+    RowSettings s;
+    s.r = p.repetition ? p.repetition[row] : p.repetition_all;
+    s.inv = 1.f / s.r;
+    s.p = p.presence ? p.presence[row] : p.presence_all;
+    s.f = p.frequency ? p.frequency[row] : p.frequency_all;
+    __syncthreads();
+    // A thread looks through every kAdjThreads-th four counts (common tokens have neighbouring numbers) and works on those with a mark, kAdjMarks at a time, over what the copy left: where out
+    // is the logits themselves, a logit that the mask allows is still there.
+    uint64_t marked = 0;                       // four bits a look
+    static_assert((kAdjLargest / 4 + kAdjThreads - 1) / kAdjThreads + 1 <= 16, "bits of a thread's counts");
+    int look = 0;
+    for (int i = tid; i < (N + p.seg) / 4; i += kAdjThreads, ++look) {
+        const uint4 n = reinterpret_cast<const uint4*>(count)[i];
+        marked |= (uint64_t)((n.x ? 1u : 0u) | (n.y ? 2u : 0u) | (n.z ? 4u : 0u) | (n.w ? 8u : 0u)) << (4 * look);
+    }
+    const int n_bias = sm_biases;
+    while (marked) {
+        int own[kAdjMarks], t[kAdjMarks], taken = 0;
+        float x[kAdjMarks];
+        bool allowed[kAdjMarks];
+#pragma unroll
+        for (int u = 0; u < kAdjMarks; ++u) {
+            if (marked) {
+                const int bit = __ffsll((long long)marked) - 1;
+                marked &= marked - 1;
+                own[u] = 4 * (tid + (bit >> 2) * kAdjThreads) + (bit & 3);
+                taken = u + 1;
+            } else {
+                own[u] = own[0];
+            }
+            t[u] = own[u] - N + v0;
+            x[u] = Pack<T>::get(in[t[u]]);
+            allowed[u] = !mask || ((mask[t[u] >> 5] >> (t[u] & 31)) & 1);
         }
-        if (mask && !((mask[i >> 5] >> (i & 31)) & 1)) x = -INFINITY;
-        out[i] = Pack<T>::put(x);
+#pragma unroll
+        for (int u = 0; u < kAdjMarks; ++u) {
+            if (u >= taken) break;
+            const uint32_t n = count[own[u]];
+            x[u] = penalized(x[u], n, s);
+            if (n & kBiased) {
+                float sum = 0.f;
+                for (int j = 0; j < n_bias; ++j)
+                    if (ids[j] == own[u]) sum += bias[j];
+                x[u] += sum;
+            }
+            out[t[u]] = Pack<T>::put(allowed[u] ? x[u] : -INFINITY);
+        }
     }
 }
 
@@ -192,18 +226,22 @@ template <typename T>
 int launch_adjust(const AdjustLogitsArgs& a, cudaStream_t stream) {
     AdjParams p = {a.logits, a.ld, a.out, a.ldo, (const long long*)a.tokens, a.ldk, a.lengths, a.prompt_lengths, a.repetition, a.presence, a.frequency, (const long long*)a.bias_ids, a.bias,
                    a.ldb, a.mask, a.ldm, a.repetition_all, a.presence_all, a.frequency_all, a.V, a.max_tokens, a.n_bias, 0};
-    // the largest segment, whose tokens are read by the fewest CTAs, that still gives every SM one
-    const int sms = sms_of_current_device();
-    p.seg = kAdjThreads * kAdjUnits * Pack<T>::N;
-    while (p.seg > 2048 && (long long)a.rows * ((a.V + p.seg - 1) / p.seg) < sms) p.seg /= 2;
-    const size_t smem = (size_t)(p.seg + 2 * Pack<T>::N + 2 * a.n_bias) * sizeof(uint32_t);
+    // Segments of a row: as few as shared memory allows, since every one reads all of the row's tokens, unless SMs would have nothing to do; then as many as the last round of CTAs has room for
+    // (64 rows of 151936: 9 of 17408 in two rounds 14 us, 10 of 16384 in three 20 us).
+    const long long slots = 2ll * sms_of_current_device();
+    long long n = ((long long)a.V + kAdjLargest - 1) / kAdjLargest;
+    const long long rounds = (a.rows * n + slots - 1) / slots, most = ((long long)a.V + 2047) / 2048;
+    n = rounds * slots / a.rows > n ? rounds * slots / a.rows : n;
+    if (n > most) n = most;
+    p.seg = (int)(((a.V + n - 1) / n + 1023) / 1024 * 1024);
     static bool once[64] = {};
     int dev = 0;
     PLZ_CUDA_CHECK(cudaGetDevice(&dev));
     if (!once[dev & 63]) {
-        PLZ_CUDA_CHECK(cudaFuncSetAttribute(adjust_logits_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, ((kAdjThreads * kAdjUnits + 2) * Pack<T>::N + 2 * kAdjBiases) * (int)sizeof(uint32_t)));
+        PLZ_CUDA_CHECK(cudaFuncSetAttribute(adjust_logits_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (kAdjLargest + Pack<T>::N) * 4 + kAdjBiases * 8));
         once[dev & 63] = true;
     }
+    const size_t smem = (a.lengths && a.max_tokens > 0) || a.n_bias > 0 ? (size_t)(p.seg + Pack<T>::N) * 4 + (size_t)a.n_bias * 8 : 0;
     PLZ_LAUNCH_CHAIN_BEHIND(adjust_logits_kernel<T>, dim3((a.V + p.seg - 1) / p.seg, a.rows), dim3(kAdjThreads), smem, stream, p);
     return PLZ_OK;
 }
