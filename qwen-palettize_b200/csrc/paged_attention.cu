@@ -572,9 +572,9 @@ int launch_paged_attn(const PagedAttnArgs& a, void* ws, long long ws_bytes, cuda
     if ((a.page_size & (a.page_size - 1)) == 0) { p.shift = 0; while ((1 << p.shift) < a.page_size) ++p.shift; }
     p.scale_log2e = a.scale * kLog2e;
     const bool wide = p.G > 8;
-    if (a.head_dim == 64) return wide ? launch_paged<Cfg<64, 16, 32, 8, 3>>(p, ctas, stream) : launch_paged<Cfg<64, 8, 32, 8, 3>>(p, ctas, stream);
-    if (a.head_dim == 128) return wide ? launch_paged<Cfg<128, 16, 16, 8, 3>>(p, ctas, stream) : launch_paged<Cfg<128, 8, 16, 8, 3>>(p, ctas, stream);
-    return wide ? launch_paged<Cfg<256, 16, 16, 4, 3>>(p, ctas, stream) : launch_paged<Cfg<256, 8, 16, 4, 3>>(p, ctas, stream);
+    if (a.head_dim == 64) return wide ? launch_paged<Cfg<64, 16, 32, 8, 2>>(p, ctas, stream) : launch_paged<Cfg<64, 8, 32, 8, 2>>(p, ctas, stream);
+    if (a.head_dim == 128) return wide ? launch_paged<Cfg<128, 16, 16, 8, 2>>(p, ctas, stream) : launch_paged<Cfg<128, 8, 16, 8, 2>>(p, ctas, stream);
+    return wide ? launch_paged<Cfg<256, 16, 16, 4, 2>>(p, ctas, stream) : launch_paged<Cfg<256, 8, 16, 4, 2>>(p, ctas, stream);
 }
 
 }  // namespace plz
