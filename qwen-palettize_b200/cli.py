@@ -39,7 +39,8 @@ def cmd_models(_args) -> int:
 def cmd_generate(args) -> int:
     from engine import Engine, SamplingParams
     prompts = [[int(t) for t in p.replace(",", " ").split()] for p in args.tokens]
-    params = SamplingParams(args.max_new, args.temperature, args.top_k, args.seed, tuple(args.stop))
+    bias = tuple((int(t), float(v)) for t, v in (b.split(":") for b in args.bias))
+    params = SamplingParams(args.max_new, args.temperature, args.top_k, args.seed, tuple(args.stop), args.repetition, args.presence, args.frequency, bias)
     eng = Engine(_load(args), max(len(p) for p in prompts) + args.max_new, args.portion, args.max_live)
     for out in eng.generate(prompts, params):
         print(" ".join(map(str, out)), flush=True)
@@ -92,6 +93,10 @@ def main(argv=None) -> int:
     g.add_argument("--top-k", type=int, default=0)
     g.add_argument("--seed", type=int, default=0)
     g.add_argument("--stop", type=int, action="append", default=[], help="token id that ends a sequence")
+    g.add_argument("--repetition", type=float, default=1.0, help="factor that makes all tokens so far less likely, 1: none")
+    g.add_argument("--presence", type=float, default=0.0, help="taken off the logits of generated tokens")
+    g.add_argument("--frequency", type=float, default=0.0, help="taken off once for every time a token was generated")
+    g.add_argument("--bias", action="append", default=[], metavar="ID:VALUE", help="added to a token's logit")
     g.add_argument("--portion", type=int, default=2048, help="most prompt tokens per step")
     g.add_argument("--max-live", type=int, default=8, help="sequences in flight")
     g.set_defaults(fn=cmd_generate)

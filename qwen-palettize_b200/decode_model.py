@@ -11,6 +11,8 @@ gate/up, SwiGLU, down, residual] -> final RMSNorm -> logits against the tied emb
                written straight into the cache by the kernels that produce them, attention over the cache, logits by the dense
                GEMM against the embedding table.  All pointers of a step are fixed once the position is known, so a step can
                be captured in a CUDA graph and replayed (decode_graph).
+  decode_paged one token per request for requests of different lengths, whose keys and values lie in the pages of a PagedKVCache.
+               Lengths, tables and positions stay on the device.
 """
 from __future__ import annotations
 
@@ -49,6 +51,49 @@ class KVCache:
     def reset(self):
         """Start over: positions at and beyond the length are never read, so nothing needs clearing."""
         self.length = 0
+
+
+class PagedKVCache:
+    """Keys and values of up to B requests of different lengths, in pages that the device hands out from one pool. A request keeps its row b of the table until it is ended."""
+
+    def __init__(self, n_layers: int, B: int, n_pages: int, page_size: int, max_tokens: int, width: int, device):
+        self.page_size = page_size
+        shape = (n_layers, n_pages, page_size, width)
+        self.k = torch.empty(shape, dtype=torch.bfloat16, device=device)      # what no request has written is never read
+        self.v = torch.empty(shape, dtype=torch.bfloat16, device=device)
+        self.table = torch.full((B, -(-max_tokens // page_size)), -1, dtype=torch.int32, device=device)
+        self.lengths = torch.zeros(B, dtype=torch.int32, device=device)
+        self.free_pages = torch.arange(n_pages, dtype=torch.int32, device=device)
+        self.n_free = torch.full((1,), n_pages, dtype=torch.int32, device=device)
+
+    @property
+    def requests(self) -> int:
+        return self.table.shape[0]
+
+    @property
+    def capacity(self) -> int:
+        """Most tokens of a request."""
+        return self.table.shape[1] * self.page_size
+
+    def plan(self, new_tokens: torch.Tensor, max_rows: int, row_pitch: int = 0) -> ops.PagePlan:
+        """Pages for the next tokens of every request (int32 [B] on the device; 0: none, negative: the request has ended and gives its pages back); the lengths
+        of the cache are those afterwards. May be captured."""
+        return ops.plan_pages(self.lengths, new_tokens, self.table, self.free_pages, self.n_free, self.page_size, max_rows, row_pitch, lengths_out=self.lengths, n_free_out=self.n_free)
+
+    def fill(self, cache: KVCache, requests) -> ops.PagePlan:
+        """The filled positions of `cache`, one sequence for each of `requests` (row numbers in increasing order) that hold nothing yet: prompts' keys and values after prefill. The plan's
+        status says who got no pages."""
+        requests = list(requests)
+        if cache.k.shape[1] != len(requests) or sorted(set(requests)) != requests or not all(0 <= r < self.requests for r in requests):
+            raise ValueError(f"{cache.k.shape[1]} sequences for the requests {requests} of {self.requests}")
+        n = cache.length
+        new = torch.zeros(self.requests, dtype=torch.int32)
+        new[requests] = n
+        p = self.plan(new.to(self.lengths.device), n * len(requests))
+        for li in range(self.k.shape[0]):
+            k, v = (t[li, :, :n].reshape(n * len(requests), -1) for t in (cache.k, cache.v))
+            ops.write_pages(k, v, p.slots, self.k[li], self.v[li])
+        return p
 
 
 class PalettizedQwen:
@@ -141,6 +186,11 @@ class PalettizedQwen:
         dev = self.embed.device
         return KVCache(torch.zeros(shape, dtype=torch.bfloat16, device=dev), torch.zeros(shape, dtype=torch.bfloat16, device=dev), 0)
 
+    def new_paged_cache(self, B: int, n_pages: int, page_size: int = 16, max_tokens: int | None = None) -> PagedKVCache:
+        """Room for B requests of up to max_tokens tokens (default: all positions of the model) that share n_pages pages."""
+        c = self.cfg
+        return PagedKVCache(c.n_layers, B, n_pages, page_size, max_tokens or self.cos.shape[0], c.n_kv_heads * c.head_dim, self.embed.device)
+
     def logits(self, h: torch.Tensor) -> torch.Tensor:
         """Final RMSNorm and the tied-embedding head: bf16 [rows, vocab]."""
         hn, _ = ops.rmsnorm_forward(h, self.final_norm, self.cfg.eps)
@@ -216,6 +266,32 @@ class PalettizedQwen:
         out = self.decode_logits(ids, cache)
         cache.length += 1
         return out
+
+    def decode_paged(self, ids: torch.Tensor, cache: PagedKVCache, new_tokens: torch.Tensor) -> torch.Tensor:
+        """One token for every request of `cache` with new_tokens[b] = 1 (int32 [B] on the device; 0: none, negative: ended): ids int64 [B] -> logits bf16 [B, vocab] of the tokens after
+        them. Rows of requests without a token, or without a page for it (the plan's status), hold nothing of use. Nothing waits for the device, so a step can be captured."""
+        c = self.cfg
+        B = cache.requests
+        if cache.capacity > self.cos.shape[0]:
+            raise ValueError(f"requests of {cache.capacity} tokens, but positions up to {self.cos.shape[0]}")
+        if ids.numel() != B or new_tokens.numel() != B:
+            raise ValueError(f"{ids.numel()} tokens and {new_tokens.numel()} counts for {B} requests")
+        p = cache.plan(new_tokens, B, row_pitch=1)
+        at = p.positions.clamp(min=0).long()
+        cos, sin = self.cos[at], self.sin[at]
+        linear = ops.hard_forward_smallm if B <= 64 else lambda w, x: ops.hard_forward(w, x)[0]
+        h = ops.embed_gather(self.embed, ids)
+        h1, _ = ops.rmsnorm_forward(h, self.layers[0]["input_ln"], c.eps)
+        n = len(self.layers)
+        for li, L in enumerate(self.layers):
+            v = linear(L["v"], h1)
+            q, k = ops.qknorm_rope_forward2(linear(L["q"], h1), L["q_norm"], c.n_heads, linear(L["k"], h1), L["k_norm"], c.n_kv_heads, cos, sin, B, c.eps)
+            ops.write_pages(k, v, p.slots, cache.k[li], cache.v[li])
+            a = ops.attention_decode_paged(q, cache.k[li], cache.v[li], cache.table, p.lengths, c.n_heads, c.n_kv_heads, c.head_dim)
+            x2, h2 = ops.add_rmsnorm_forward(h, linear(L["o"], a), L["post_ln"], c.eps)
+            d = linear(L["down"], ops.swiglu_forward(linear(L["gate"], h2), linear(L["up"], h2)))
+            h, h1 = ops.add_rmsnorm_forward(x2, d, self.layers[li + 1]["input_ln"] if li + 1 < n else self.final_norm, c.eps)
+        return self.head(h1)
 
     def decode_graph(self, ids: torch.Tensor, cache: KVCache, pos: int):
         """A CUDA graph of one decode step at a fixed position (ids is read at replay, so the caller may overwrite it in place

@@ -21,6 +21,14 @@ class SamplingParams:
     top_k: int = 0               # 0: all tokens
     seed: int = 0
     stop: tuple = ()             # token ids that end the request (kept in the output)
+    repetition: float = 1.0      # what the logits of all tokens so far are divided by (negative ones: multiplied)
+    presence: float = 0.0        # taken off the logits of generated tokens,
+    frequency: float = 0.0       # and as often as they were generated
+    bias: tuple = ()             # (token id, added to its logit) pairs
+    allowed: object = None       # callable: generated tokens so far -> ids that may come next, None: all
+
+    def adjusts(self) -> bool:
+        return self.repetition != 1.0 or self.presence != 0.0 or self.frequency != 0.0 or bool(self.bias) or self.allowed is not None
 
 
 @dataclass
@@ -31,6 +39,8 @@ class Request:
     fed: int = 0                                   # prompt tokens already run
     out: list = field(default_factory=list)
     done: bool = False
+    said: torch.Tensor | None = None               # prompt and generated tokens on the device, for the penalties
+    bias: tuple | None = None                      # (ids, values) on the device
 
 
 class Engine:
@@ -69,6 +79,10 @@ class Engine:
         params = params or SamplingParams()
         if not prompt:
             raise ValueError("empty prompt")
+        if not params.repetition > 0.0:
+            raise ValueError("the repetition penalty is a positive factor")
+        if any(not 0 <= t < self.model.vocab for t, _ in params.bias):
+            raise ValueError(f"a bias for a token outside the vocabulary of {self.model.vocab}")
         if len(prompt) + params.max_new > self.pool.capacity:
             raise ValueError(f"{len(prompt)} + {params.max_new} tokens exceed the capacity {self.pool.capacity}")
         rid = ("gen", self._next)
@@ -111,9 +125,37 @@ class Engine:
     def _take(self, r: Request, logits: torch.Tensor):
         p = r.params
         at = torch.tensor([r.fed + len(r.out)], dtype=torch.int32, device=logits.device)
+        if p.adjusts():
+            logits = self._adjust(r, logits)
         tok = int(S.sample(logits, at, p.temperature, p.top_k, p.seed).item())
         r.out.append(tok)
         r.done = tok in p.stop
+
+    def _adjust(self, r: Request, logits: torch.Tensor) -> torch.Tensor:
+        """The request's settings on its logits fp32 [1, V]."""
+        p, dev, V = r.params, logits.device, logits.shape[1]
+        kw = {}
+        if p.repetition != 1.0 or p.presence != 0.0 or p.frequency != 0.0:
+            n, n_prompt = len(r.prompt) + len(r.out), len(r.prompt)
+            if r.said is None:
+                r.said = torch.tensor([r.prompt + [0] * p.max_new], dtype=torch.int64, device=dev)
+            if r.out:
+                S.put(r.said[0, n - 1:n], torch.tensor(r.out[-1:]))
+            counts = torch.tensor([[n], [n_prompt]], dtype=torch.int32, device=dev)
+            kw = dict(tokens=r.said, lengths=counts[0], prompt_lengths=counts[1], repetition=p.repetition, presence=p.presence, frequency=p.frequency)
+        if p.bias:
+            if r.bias is None:
+                r.bias = (torch.tensor([[t for t, _ in p.bias]], dtype=torch.int64, device=dev), torch.tensor([[b for _, b in p.bias]], dtype=torch.float32, device=dev))
+            kw.update(bias_ids=r.bias[0], bias=r.bias[1])
+        ids = p.allowed(list(r.out)) if p.allowed is not None else None
+        if ids is not None:
+            ids = torch.tensor(sorted(set(ids)), dtype=torch.int64)
+            if ids.numel() == 0 or ids[0] < 0 or ids[-1] >= V:
+                raise ValueError(f"request {r.rid!r}: no token is allowed, or one outside the vocabulary of {V}")
+            words = torch.zeros((V + 31) // 32, dtype=torch.int64)
+            words.index_add_(0, ids >> 5, 1 << (ids & 31))
+            kw["mask"] = torch.where(words >= 1 << 31, words - (1 << 32), words).to(torch.int32).view(1, -1).to(dev)
+        return S.adjust_logits(logits, **kw)
 
     def run(self) -> dict:
         """Until every submitted request is finished: {request id: generated tokens} of all finished so far."""

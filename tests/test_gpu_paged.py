@@ -356,3 +356,61 @@ def test_pool_past_four_gigabytes():
     got = ops.attention_decode_paged(q, kp, vp, ids, _dev([n]), 8, 2)
     small = [t[ids[0].long()].contiguous() for t in (kp, vp)]
     _close(got, *ref.attention(q, *small, _dev([[0, 1, 2, 3]]), _dev([n]), 8, 2, 128))
+
+
+# ---- the calls from Python -----------------------------------------------------------------------------------------------------
+class _Declines:
+    """In place of the native calls: declines everything, so that the general path runs."""
+    def __getattr__(self, name):
+        return lambda *a: None
+
+
+def test_general_path_and_native_calls_agree(monkeypatch):
+    import plz_native as P
+    import plz_ops as ops
+    import seq_ops as S
+
+    def everything():
+        cached, new, table, free, n_free = _requests(5, 30, 16, 100, 9, spare=60, ended=0.1)
+        tab, F = _dev(table), _dev(free)
+        p = ops.plan_pages(_dev(cached), _dev(new), tab, F, _dev([n_free]), 16, 200)
+        q, kp, vp, t2, L = _case(4, RAGGED, 8, 2, 128, 16, fill=0.0)
+        k = torch.arange(13 * 256, device="cuda").view(13, 256).bfloat16()
+        slots = torch.arange(13, device="cuda", dtype=I32) * 3 - 1
+        ops.write_pages(k, k * 2, slots, kp, vp)
+        out = torch.zeros(13, 1104, dtype=torch.bfloat16, device="cuda")[:, 8:1032]
+        bad = torch.zeros(1, dtype=I32, device="cuda")
+        o1, o2 = ops.attention_decode_paged(q, kp, vp, t2, L, 8, 2), ops.attention_decode_paged(q, kp, vp, t2, L, 8, 2, 128, 0.5, out, bad)
+        g = torch.Generator(device="cuda").manual_seed(1)
+        x = torch.randn(3, 500, generator=g, device="cuda")
+        tok = torch.randint(0, 500, (3, 40), generator=g, device="cuda")
+        one = torch.full((3,), 1.5, device="cuda")
+        kw = dict(tokens=tok, lengths=_dev([40, 3, 0]), prompt_lengths=_dev([4, 0, 1]), repetition=one, presence=0.5, frequency=0, bias_ids=tok[:, :7].contiguous(), bias=torch.randn(3, 7, generator=g, device="cuda"),
+                  mask=torch.randint(-2 ** 31, 2 ** 31, (1, 16), generator=g, device="cuda").int())
+        y1, y2 = S.adjust_logits(x, **kw), S.adjust_logits(x.bfloat16(), presence=0.25, tokens=tok, lengths=_dev([40, 3, 0]))
+        y3 = S.adjust_logits(x, out=torch.empty_like(x))
+        return [p.lengths, p.n_free, p.starts, p.slots, p.positions, p.status, tab, F, kp, vp, o1, o2, out.clone(), bad, y1, y2, y3]
+    native = everything()
+    calls = P.calls()
+    for name in ("plan_pages", "write_pages", "attention_decode_paged", "adjust_logits"):
+        assert getattr(calls, name)() is None
+    monkeypatch.setattr(P, "calls", lambda: _Declines())
+    general = everything()
+    assert all(torch.equal(a, b) for a, b in zip(native, general))
+    # a tensor on another device than the current one is refused ahead of any launch
+    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: 1)
+    with pytest.raises(P.PlzError, match="current device"):
+        everything()
+
+
+def test_results_that_are_written_past_are_refused():
+    import plz_native as P
+    import plz_ops as ops
+    q, kp, vp, table, L = _case(1, [5], 8, 2, 128, 16)
+    with pytest.raises(P.PlzError):
+        ops.attention_decode_paged(q, kp, vp, table, L, 8, 2, out=q)
+    new = _dev([1])
+    with pytest.raises(P.PlzError):
+        ops.plan_pages(L, new, table, _dev([0]), _dev([1]), 16, 1, lengths_out=new)
+    with pytest.raises(P.PlzError):          # rows that are no whole 16-byte units
+        ops.write_pages(kp[0, :, :100], vp[0, :, :100], _dev([-1] * 16), kp[:, :, :100], vp[:, :, :100])

@@ -28,6 +28,7 @@ def test_page_plan_refusals(built_lib):
     for kw in ({"B": 16385}, {"width": 1 << 28, "ldt": 1 << 28}, {"n_pages": 1 << 27}, {"max_rows": (1 << 30) + 1}):
         assert call(**kw) == LARGE, kw
     assert b"16384" in P.lib().plz_last_error()
+    assert call(lengths=base["new_tokens"]) == UNSUPPORTED
 
 
 def test_page_write_refusals(built_lib):
