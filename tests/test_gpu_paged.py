@@ -123,7 +123,7 @@ def test_planned_steps_captured():
 
 
 # ---- rows -----------------------------------------------------------------------------------------------------------------
-@pytest.mark.parametrize("rows,width,page,dtype", [(1, 8, 1, torch.bfloat16), (7, 40, 16, torch.bfloat16), (64, 1024, 16, torch.bfloat16), (100, 24, 5, torch.float32), (9000, 128, 64, torch.bfloat16),
+@pytest.mark.parametrize("rows,width,page,dtype", [(1, 8, 1, torch.bfloat16), (7, 40, 16, torch.bfloat16), (64, 1024, 16, torch.bfloat16), (100, 24, 5, torch.float32), (9000, 128, 64, torch.bfloat16), (9001, 1024, 16, torch.bfloat16),
                                                    (3001, 520, 24, torch.float32), (33, 4096, 8, torch.uint8)])
 @pytest.mark.parametrize("strided", [False, True])
 def test_write(rows, width, page, dtype, strided):
