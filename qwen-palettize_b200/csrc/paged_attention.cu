@@ -2,22 +2,27 @@
 //
 // Bound by memory: a cached token and key / value head is 4 * head_dim bytes that are read once, for the 4 * G * head_dim operations of the G query heads that share them.
 //
-//   paged_attn_kernel  One CTA per SM. The work is a line of steps of 16 tokens: requests in order, in each its key / value heads (and blocks of 16 query heads), in each its
-//     tokens. Every warp takes an equal stretch of the line, whatever the lengths are: it finds its first request by a sum over the lengths that its CTA makes. A warp asks for its
-//     steps NST ahead with 16-byte cp.async copies through a ring of its own, which goes on over the ends of heads and requests, so nothing waits between short requests and there is no
-//     barrier until a CTA's warps meet at the end. Scores and sums are mma.sync m16n8k16 on fragments read by ldmatrix: the query heads are the 16 rows, the tokens the columns. (tcgen05 has
-//     64 rows at least, for 4 query heads here, and would need the warps to meet in every step; with 4 heads the products use an eighth of what mma.sync offers at the speed of memory.)
+//   paged_attn_kernel  One CTA per SM. The work is a line of steps of 16 tokens (32 of 64-wide heads): requests in order, in each its key / value heads (and blocks of 16 query heads), in each
+//     its tokens. Every warp takes an equal stretch of the line, whatever the lengths are: it finds its first request by a sum over the lengths that its CTA makes. The pages of a step's
+//     tokens are asked for four steps ahead, its keys and values two steps ahead, all by cp.async through a ring of the warp's own, which goes on over the ends of heads and requests: nothing waits
+//     between short requests, and there is no barrier until a CTA's warps meet at the end.
+//     Scores and sums are mma.sync m16n8k16 on fragments read by ldmatrix: the query heads are the 16 rows, the tokens the columns. tcgen05 has 64 rows at least, for the 4 query heads of
+//     a group here, and would need the warps to meet in every step; the tensor pipe is 19 % busy at the speed of memory as it is.
 //     Weights are two bf16 terms, high and low part, of the fp32 value: 16 bits of it enter the product, so the result is as exact as its own rounding to bf16. With up to 8 query heads
-//     the low parts are rows 8 to 15 of the same product and cost nothing.
-//     The reference of the exponentials moves when a row's maximum has grown by more than 2^8.
+//     the low parts are rows 8 to 15 of the same product and cost nothing. The reference of the exponentials moves when a row's maximum has grown by more than 2^8.
 //     A head that a warp finishes alone goes to `out`; parts meet in shared memory at the end, parts that cross CTAs go to the workspace, two per CTA at most.
-//   paged_join_kernel  one CTA per CTA of the first kernel joins the parts of the head that began there and went on; most have nothing to do.
+//   paged_join_kernel  one block per CTA of the first kernel and query head of a group joins the parts of the head that began there and went on; most have nothing to do.
+//
+// Measured (query / key heads 32 / 8 of 128, pages of 16 or 64): 2 x 131072 tokens 160 us for 1.07 GB, 6.7 TB/s; 64 requests of up to 4096 tokens 96 us for 0.59 GB, 6.1 TB/s; 256 requests of up to
+// 300 tokens, 16 / 16 heads of 64, 37 us for 0.16 GB; one request of 2049 tokens 9 us, a chain of latencies: lengths, pages, keys, two meetings, a second launch.
+//   What is in flight matters: three steps a warp (196 KB of copies per SM) 187 and 110 us, since SMs then starve one another (their times spread over 73 to 95 us at equal work, which taking the
+//   work as it comes did not mend: its many parts cost as much as it gave); two steps (128 KB) 160 and 96; six warps of two steps 166 and 100.
 #include "plz_launch.h"
 
 namespace plz {
 namespace {
 
-constexpr int kSwitch = 2;               // steps that the change to another head counts on the line
+constexpr int kSwitch = 2;               // steps that the change to another head counts on the line (0: 256 short requests 45 us; 1, 2: 37; 4: 39)
 constexpr float kGrow = 8.f;             // exponents (base 2) that a maximum may grow before the reference moves
 constexpr float kLog2e = 1.4426950408889634f;
 
@@ -571,6 +576,7 @@ int launch_paged_attn(const PagedAttnArgs& a, void* ws, long long ws_bytes, cuda
     p.shift = -1;
     if ((a.page_size & (a.page_size - 1)) == 0) { p.shift = 0; while ((1 << p.shift) < a.page_size) ++p.shift; }
     p.scale_log2e = a.scale * kLog2e;
+    // more than eight query heads share a key: the low parts of the weights are a product of their own
     const bool wide = p.G > 8;
     if (a.head_dim == 64) return wide ? launch_paged<Cfg<64, 16, 32, 8, 2>>(p, ctas, stream) : launch_paged<Cfg<64, 8, 32, 8, 2>>(p, ctas, stream);
     if (a.head_dim == 128) return wide ? launch_paged<Cfg<128, 16, 16, 8, 2>>(p, ctas, stream) : launch_paged<Cfg<128, 8, 16, 8, 2>>(p, ctas, stream);
