@@ -7,16 +7,21 @@
 //   A CTA takes a segment of a row, copies it through the mask, 16 bytes a thread and access, and counts the row's tokens that fall into it in shared memory (whole numbers, exact in any order);
 //   reading all tokens in every CTA costs less than a cluster that reads them once and counts in its distributed shared memory (8 rows with 30000 tokens 18 us, 64 rows 38 us: its CTAs wait for one
 //   another, and its atomics are slow). One warp lists the biases of the segment's tokens in their order and marks the tokens' counts; several biases of one token are added in the order of
-//   the row's list whatever the threads do. Then the marked logits are computed and stored over the copy.
+//   the row's list whatever the threads do. Then the tokens with a mark are listed, their logits computed by all threads alike and stored over the copy.
 #include "plz_launch.h"
 
 namespace plz {
 namespace {
 
-constexpr int kAdjUnits = 2, kAdjTokens = 8, kAdjMarks = 4;      // 16-byte units, tokens, marked logits of a thread that are on their way at once
-constexpr int kAdjPerThread = 40;                     // logits of a CTA at most, per thread (160 KB of counts per SM with 1024 threads)
+constexpr int kAdjFirst = 2, kAdjUnits = 4, kAdjTokens = 8, kAdjMarks = 4;      // 16-byte units (first ones, later ones), tokens, marked logits of a thread that are on their way at once
+// logits of a CTA of 512 threads (counts of 16 bits, histories of up to 8192 tokens) and of 1024 (of 32 bits) at most: what shared memory holds of counts, list and biases
+constexpr int kAdjLargest = 40960, kAdjLargestLong = 32768, kAdjShort = 8192;
 constexpr int kAdjBiases = 4096;         // of a row at most
-constexpr uint32_t kSeen = 0x80000000u, kBiased = 0x40000000u, kCount = 0x3FFFFFFFu;
+
+// a token's mark: occurs, has a bias, how often behind the prompt
+template <bool SHORT> struct Mark;
+template <> struct Mark<false> { static constexpr uint32_t kSeen = 0x80000000u, kBiased = 0x40000000u, kCount = 0x3FFFFFFFu; };
+template <> struct Mark<true> { static constexpr uint32_t kSeen = 0x8000u, kBiased = 0x4000u, kCount = 0x3FFFu; };
 
 struct AdjParams {
     const void* in; long long ld;
@@ -50,9 +55,10 @@ template <> struct Pack<__nv_bfloat16> {
 
 struct RowSettings { float r, inv, p, f; };      // inv = 1 / r: x * inv is within 2^-23 of x / r
 
+template <typename M>
 __device__ __forceinline__ float penalized(float x, uint32_t n, const RowSettings& s) {
-    const uint32_t c = n & kCount;
-    if (n & (kSeen | kCount)) x *= x > 0.f ? s.inv : s.r;
+    const uint32_t c = n & M::kCount;
+    if (n & (M::kSeen | M::kCount)) x *= x > 0.f ? s.inv : s.r;
     return c ? x - s.f * (float)c - s.p : x;
 }
 
@@ -62,10 +68,21 @@ template <typename T, int kAdjThreads>
 __global__ void __launch_bounds__(kAdjThreads, 1024 / kAdjThreads)
 adjust_logits_kernel(const AdjParams p) {
     constexpr int N = Pack<T>::N;
-    extern __shared__ __align__(16) uint32_t count[];                       // [N + seg]
-    __shared__ int sm_biases;
-    int* const ids = reinterpret_cast<int*>(count + N + p.seg);            // biases of this CTA's tokens
+    constexpr bool SHORT = kAdjThreads == 512;
+    constexpr int PER = SHORT ? 8 : 4;                                      // counts in 16 bytes
+    typedef Mark<SHORT> M;
+    extern __shared__ __align__(16) uint32_t count[];                       // N + seg counts, of 16 bits two a word
+    const int words16 = (N + p.seg + PER - 1) / PER;                        // 16-byte words of them
+    auto mark = [&](int own, uint32_t what, bool add) {
+        uint32_t* const where = SHORT ? count + own / 2 : count + own;
+        if (SHORT) what <<= (own & 1) * 16;
+        if (add) atomicAdd(where, what); else atomicOr(where, what);
+    };
+    auto marked = [&](int own) { return SHORT ? (uint32_t)reinterpret_cast<const uint16_t*>(count)[own] : count[own]; };
+    __shared__ int sm_list, sm_biases;
+    int* const ids = reinterpret_cast<int*>(count + words16 * 4);           // biases of this CTA's tokens
     float* const bias = reinterpret_cast<float*>(ids + p.n_bias);
+    uint16_t* const list = reinterpret_cast<uint16_t*>(bias + p.n_bias);   // own numbers of the tokens with a mark
     const int row = blockIdx.y, tid = threadIdx.x, lane = tid & 31;
     const T* in = (const T*)p.in + row * p.ld;
     T* out = (T*)p.out + row * p.ldo;
@@ -73,8 +90,8 @@ adjust_logits_kernel(const AdjParams p) {
     const int v0 = min(head + (int)blockIdx.x * p.seg, p.V), s0 = blockIdx.x ? v0 : 0, s1 = blockIdx.x + 1 == gridDim.x ? p.V : min(v0 + p.seg, p.V);
     const bool vec = (((uintptr_t)(out + head)) & 15) == 0, marks = (p.lengths && p.max_tokens > 0) || p.n_bias > 0;
     if (marks) {
-        for (int i = tid; i < (N + p.seg) / 4; i += kAdjThreads) reinterpret_cast<uint4*>(count)[i] = make_uint4(0u, 0u, 0u, 0u);
-        if (tid == 0) sm_biases = 0;
+        for (int i = tid; i < words16; i += kAdjThreads) reinterpret_cast<uint4*>(count)[i] = make_uint4(0u, 0u, 0u, 0u);
+        if (tid == 0) sm_list = sm_biases = 0;
     }
     pdl_launch_dependents();
     pdl_wait();
@@ -92,9 +109,9 @@ adjust_logits_kernel(const AdjParams p) {
             u.hi = mask[min(w + 1, words - 1)];
         }
     };
-    Unit unit[kAdjUnits];                      // the first ones are on their way while tokens are counted
+    Unit first[kAdjFirst];                     // on their way while tokens are counted
 #pragma unroll
-    for (int k = 0; k < kAdjUnits; ++k) load(v0 + (k * kAdjThreads + tid) * N, unit[k]);
+    for (int k = 0; k < kAdjFirst; ++k) load(v0 + (k * kAdjThreads + tid) * N, first[k]);
     if (marks) {
         // the first tokens are asked for ahead of knowing how many there are
         const int most = p.lengths ? p.max_tokens : 0;
@@ -135,7 +152,7 @@ adjust_logits_kernel(const AdjParams p) {
                         const int at = n + __popc(all & ((1u << lane) - 1u));
                         ids[at] = own;
                         bias[at] = v[u];
-                        atomicOr(count + own, kBiased);
+                        mark(own, M::kBiased, false);
                     }
                     n += __popc(all);
                 }
@@ -147,30 +164,31 @@ adjust_logits_kernel(const AdjParams p) {
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 if (t[u] < s0 || t[u] >= s1 || i0 + u * kAdjThreads >= n_tok) continue;
-                uint32_t* const where = count + N + (int)t[u] - v0;
-                if (i0 + u * kAdjThreads < n_prompt) atomicOr(where, kSeen); else atomicAdd(where, 1u);
+                const bool own_word = i0 + u * kAdjThreads >= n_prompt;
+                mark(N + (int)t[u] - v0, own_word ? 1u : M::kSeen, own_word);
             }
             fetch(i0 + kAdjThreads * U);
         }
     }
-    // all logits, kAdjUnits units of a thread at a time
-    for (int t0 = v0; t0 < s1; t0 += kAdjUnits * kAdjThreads * N) {
-        if (t0 > v0) {
-#pragma unroll
-            for (int k = 0; k < kAdjUnits; ++k) load(t0 + (k * kAdjThreads + tid) * N, unit[k]);
+    // all logits
+    auto store = [&](int t, Unit& u) {
+        if (t >= s1) return;
+        if (vec && t + N <= s1) {
+            if (mask) u.raw = Pack<T>::masked(u.raw, __funnelshift_r(u.lo, u.hi, t & 31));
+            *reinterpret_cast<uint4*>(out + t) = u.raw;
+        } else {
+            // the row's end, or in and out lie differently
+            for (int e = 0; e < N && t + e < s1; ++e) out[t + e] = !mask || ((mask[(t + e) >> 5] >> ((t + e) & 31)) & 1) ? in[t + e] : Pack<T>::put(-INFINITY);
         }
+    };
 #pragma unroll
-        for (int k = 0; k < kAdjUnits; ++k) {
-            const int t = t0 + (k * kAdjThreads + tid) * N;
-            if (t >= s1) continue;
-            if (vec && t + N <= s1) {
-                if (mask) unit[k].raw = Pack<T>::masked(unit[k].raw, __funnelshift_r(unit[k].lo, unit[k].hi, t & 31));
-                *reinterpret_cast<uint4*>(out + t) = unit[k].raw;
-            } else {
-                // the row's end, or in and out lie differently
-                for (int e = 0; e < N && t + e < s1; ++e) out[t + e] = !mask || ((mask[(t + e) >> 5] >> ((t + e) & 31)) & 1) ? in[t + e] : Pack<T>::put(-INFINITY);
-            }
-        }
+    for (int k = 0; k < kAdjFirst; ++k) store(v0 + (k * kAdjThreads + tid) * N, first[k]);
+    for (int t0 = v0 + kAdjFirst * kAdjThreads * N; t0 < s1; t0 += kAdjUnits * kAdjThreads * N) {
+        Unit unit[kAdjUnits];
+#pragma unroll
+        for (int k = 0; k < kAdjUnits; ++k) load(t0 + (k * kAdjThreads + tid) * N, unit[k]);
+#pragma unroll
+        for (int k = 0; k < kAdjUnits; ++k) store(t0 + (k * kAdjThreads + tid) * N, unit[k]);
     }
     if (tid < v0 - s0) out[tid] = !mask || ((mask[0] >> tid) & 1) ? in[tid] : Pack<T>::put(-INFINITY);
     if (!marks) return;
@@ -180,59 +198,80 @@ adjust_logits_kernel(const AdjParams p) {
     s.p = p.presence ? p.presence[row] : p.presence_all;
     s.f = p.frequency ? p.frequency[row] : p.frequency_all;
     __syncthreads();
-    // A thread looks through every kAdjThreads-th four counts (common tokens have neighbouring numbers) and works on those with a mark, kAdjMarks at a time, over what the copy left: where out
-    // is the logits themselves, a logit that the mask allows is still there.
-    uint64_t marked = 0;                       // four bits a look
-    static_assert(kAdjPerThread / 4 + 1 <= 16, "bits of a thread's counts");
-    int look = 0;
-    for (int i = tid; i < (N + p.seg) / 4; i += kAdjThreads, ++look) {
+    // The tokens with a mark are listed, so that the work on them is spread over all threads: every kAdjThreads-th 16 bytes of counts are a thread's.
+    constexpr int kLooks = ((SHORT ? kAdjLargest : kAdjLargestLong) + N) / PER / kAdjThreads + 1;
+    uint32_t found[(kLooks + 3) / 4];          // eight bits a look
+#pragma unroll
+    for (int l = 0; l < (kLooks + 3) / 4; ++l) found[l] = 0u;
+    int k = 0;
+#pragma unroll
+    for (int look = 0; look < kLooks; ++look) {
+        const int i = tid + look * kAdjThreads;
+        if (i >= words16) break;
         const uint4 n = reinterpret_cast<const uint4*>(count)[i];
-        marked |= (uint64_t)((n.x ? 1u : 0u) | (n.y ? 2u : 0u) | (n.z ? 4u : 0u) | (n.w ? 8u : 0u)) << (4 * look);
+        uint32_t bits;
+        if (SHORT)
+            bits = ((n.x & 0xFFFFu) ? 1u : 0u) | (n.x >> 16 ? 2u : 0u) | ((n.y & 0xFFFFu) ? 4u : 0u) | (n.y >> 16 ? 8u : 0u) | ((n.z & 0xFFFFu) ? 16u : 0u) | (n.z >> 16 ? 32u : 0u) |
+                   ((n.w & 0xFFFFu) ? 64u : 0u) | (n.w >> 16 ? 128u : 0u);
+        else
+            bits = (n.x ? 1u : 0u) | (n.y ? 2u : 0u) | (n.z ? 4u : 0u) | (n.w ? 8u : 0u);
+        found[look / 4] |= bits << (look % 4 * 8);
+        k += __popc(bits);
     }
-    const int n_bias = sm_biases;
-    while (marked) {
-        int own[kAdjMarks], t[kAdjMarks], taken = 0;
+    int upto = k, base = 0;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int up = __shfl_up_sync(0xFFFFFFFFu, upto, o);
+        if (lane >= o) upto += up;
+    }
+    if (lane == 31 && upto) base = atomicAdd(&sm_list, upto);
+    base = __shfl_sync(0xFFFFFFFFu, base, 31) + upto - k;
+#pragma unroll
+    for (int l = 0; l < (kLooks + 3) / 4; ++l)
+        for (uint32_t left = found[l]; left; left &= left - 1u) {
+            const int bit = __ffs(left) - 1;
+            list[base++] = (uint16_t)(PER * (tid + (4 * l + (bit >> 3)) * kAdjThreads) + (bit & 7));
+        }
+    __syncthreads();
+    // Their results over what the copy left: where out is the logits themselves, a logit that the mask allows is still there.
+    const int n_list = sm_list, n_bias = sm_biases;
+    for (int i0 = tid; i0 < n_list; i0 += kAdjThreads * kAdjMarks) {
+        int own[kAdjMarks];
         float x[kAdjMarks];
         bool allowed[kAdjMarks];
 #pragma unroll
         for (int u = 0; u < kAdjMarks; ++u) {
-            if (marked) {
-                const int bit = __ffsll((long long)marked) - 1;
-                marked &= marked - 1;
-                own[u] = 4 * (tid + (bit >> 2) * kAdjThreads) + (bit & 3);
-                taken = u + 1;
-            } else {
-                own[u] = own[0];
-            }
-            t[u] = own[u] - N + v0;
-            x[u] = Pack<T>::get(in[t[u]]);
-            allowed[u] = !mask || ((mask[t[u] >> 5] >> (t[u] & 31)) & 1);
+            if (i0 + u * kAdjThreads >= n_list) break;
+            own[u] = list[i0 + u * kAdjThreads];
+            const int t = own[u] - N + v0;
+            x[u] = Pack<T>::get(in[t]);
+            allowed[u] = !mask || ((mask[t >> 5] >> (t & 31)) & 1);
         }
 #pragma unroll
         for (int u = 0; u < kAdjMarks; ++u) {
-            if (u >= taken) break;
-            const uint32_t n = count[own[u]];
-            x[u] = penalized(x[u], n, s);
-            if (n & kBiased) {
+            if (i0 + u * kAdjThreads >= n_list) break;
+            const uint32_t n = marked(own[u]);
+            float y = penalized<M>(x[u], n, s);
+            if (n & M::kBiased) {
                 float sum = 0.f;
                 for (int j = 0; j < n_bias; ++j)
                     if (ids[j] == own[u]) sum += bias[j];
-                x[u] += sum;
+                y += sum;
             }
-            out[t[u]] = Pack<T>::put(allowed[u] ? x[u] : -INFINITY);
+            out[own[u] - N + v0] = Pack<T>::put(allowed[u] ? y : -INFINITY);
         }
     }
 }
 
 template <typename T, int kAdjThreads>
 int launch_adjust(const AdjustLogitsArgs& a, cudaStream_t stream) {
-    constexpr int kAdjLargest = kAdjPerThread * kAdjThreads;
+    constexpr int kLargest = kAdjThreads == 512 ? kAdjLargest : kAdjLargestLong;
     AdjParams p = {a.logits, a.ld, a.out, a.ldo, (const long long*)a.tokens, a.ldk, a.lengths, a.prompt_lengths, a.repetition, a.presence, a.frequency, (const long long*)a.bias_ids, a.bias,
                    a.ldb, a.mask, a.ldm, a.repetition_all, a.presence_all, a.frequency_all, a.V, a.max_tokens, a.n_bias, 0};
     // Segments of a row: as few as shared memory allows, since every one reads all of the row's tokens, unless SMs would have nothing to do; then as many as the last round of CTAs has room for
     // (64 rows of 151936: 9 of 17408 in two rounds 14 us, 10 of 16384 in three 20 us).
     const long long slots = 1024ll / kAdjThreads * sms_of_current_device();
-    long long n = ((long long)a.V + kAdjLargest - 1) / kAdjLargest;
+    long long n = ((long long)a.V + kLargest - 1) / kLargest;
     const long long rounds = (a.rows * n + slots - 1) / slots, most = ((long long)a.V + 2047) / 2048;
     n = rounds * slots / a.rows > n ? rounds * slots / a.rows : n;
     if (n > most) n = most;
@@ -241,10 +280,11 @@ int launch_adjust(const AdjustLogitsArgs& a, cudaStream_t stream) {
     int dev = 0;
     PLZ_CUDA_CHECK(cudaGetDevice(&dev));
     if (!once[dev & 63]) {
-        PLZ_CUDA_CHECK(cudaFuncSetAttribute((adjust_logits_kernel<T, kAdjThreads>), cudaFuncAttributeMaxDynamicSharedMemorySize, (kAdjLargest + Pack<T>::N) * 4 + kAdjBiases * 8));
+        PLZ_CUDA_CHECK(cudaFuncSetAttribute((adjust_logits_kernel<T, kAdjThreads>), cudaFuncAttributeMaxDynamicSharedMemorySize, (kLargest + 16) * (kAdjThreads == 512 ? 4 : 6) + kAdjBiases * 8));
         once[dev & 63] = true;
     }
-    const size_t smem = (a.lengths && a.max_tokens > 0) || a.n_bias > 0 ? (size_t)(p.seg + Pack<T>::N) * 4 + (size_t)a.n_bias * 8 : 0;
+    const long long listed = (a.lengths ? (long long)a.max_tokens : 0) + a.n_bias, room = listed < p.seg + Pack<T>::N ? listed : p.seg + Pack<T>::N;
+    const size_t smem = (a.lengths && a.max_tokens > 0) || a.n_bias > 0 ? (size_t)(p.seg + 8) * (kAdjThreads == 512 ? 2 : 4) + (size_t)a.n_bias * 8 + (size_t)room * 2 : 0;
     PLZ_LAUNCH_CHAIN_BEHIND((adjust_logits_kernel<T, kAdjThreads>), dim3((a.V + p.seg - 1) / p.seg, a.rows), dim3(kAdjThreads), smem, stream, p);
     return PLZ_OK;
 }
@@ -253,7 +293,7 @@ int launch_adjust(const AdjustLogitsArgs& a, cudaStream_t stream) {
 
 int launch_adjust_logits(int dtype, const AdjustLogitsArgs& a, cudaStream_t stream) {
     // Long histories, which every CTA of a row reads, are read by fewer CTAs of twice the threads (8 rows of 151936 with 30000 tokens 13.3 -> 11.1 us; 64 rows with 4096 tokens 18.7, 20.9 that way).
-    if (a.lengths && a.max_tokens > 8192) return dtype == 1 ? launch_adjust<float, 1024>(a, stream) : launch_adjust<__nv_bfloat16, 1024>(a, stream);
+    if (a.lengths && a.max_tokens > kAdjShort) return dtype == 1 ? launch_adjust<float, 1024>(a, stream) : launch_adjust<__nv_bfloat16, 1024>(a, stream);
     return dtype == 1 ? launch_adjust<float, 512>(a, stream) : launch_adjust<__nv_bfloat16, 512>(a, stream);
 }
 
