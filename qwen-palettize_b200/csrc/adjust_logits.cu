@@ -13,7 +13,7 @@
 namespace plz {
 namespace {
 
-constexpr int kAdjFirst = 2, kAdjUnits = 4, kAdjTokens = 8, kAdjMarks = 4;      // 16-byte units (first ones, later ones), tokens, marked logits of a thread that are on their way at once
+constexpr int kAdjFirst = 2, kAdjUnits = 4, kAdjTokens = 8;      // 16-byte units (first ones, later ones) and tokens of a thread that are on their way at once
 // logits of a CTA of 512 threads (counts of 16 bits, histories of up to 8192 tokens) and of 1024 (of 32 bits) at most: what shared memory holds of counts, list and biases
 constexpr int kAdjLargest = 40960, kAdjLargestLong = 32768, kAdjShort = 8192;
 constexpr int kAdjBiases = 4096;         // of a row at most
@@ -235,31 +235,19 @@ adjust_logits_kernel(const AdjParams p) {
     __syncthreads();
     // Their results over what the copy left: where out is the logits themselves, a logit that the mask allows is still there.
     const int n_list = sm_list, n_bias = sm_biases;
-    for (int i0 = tid; i0 < n_list; i0 += kAdjThreads * kAdjMarks) {
-        int own[kAdjMarks];
-        float x[kAdjMarks];
-        bool allowed[kAdjMarks];
-#pragma unroll
-        for (int u = 0; u < kAdjMarks; ++u) {
-            if (i0 + u * kAdjThreads >= n_list) break;
-            own[u] = list[i0 + u * kAdjThreads];
-            const int t = own[u] - N + v0;
-            x[u] = Pack<T>::get(in[t]);
-            allowed[u] = !mask || ((mask[t >> 5] >> (t & 31)) & 1);
+    for (int i = tid; i < n_list; i += kAdjThreads) {
+        const int own = list[i], t = own - N + v0;
+        const float x = Pack<T>::get(in[t]);
+        const bool allowed = !mask || ((mask[t >> 5] >> (t & 31)) & 1);
+        const uint32_t n = marked(own);
+        float y = penalized<M>(x, n, s);
+        if (n & M::kBiased) {
+            float sum = 0.f;
+            for (int j = 0; j < n_bias; ++j)
+                if (ids[j] == own) sum += bias[j];
+            y += sum;
         }
-#pragma unroll
-        for (int u = 0; u < kAdjMarks; ++u) {
-            if (i0 + u * kAdjThreads >= n_list) break;
-            const uint32_t n = marked(own[u]);
-            float y = penalized<M>(x[u], n, s);
-            if (n & M::kBiased) {
-                float sum = 0.f;
-                for (int j = 0; j < n_bias; ++j)
-                    if (ids[j] == own[u]) sum += bias[j];
-                y += sum;
-            }
-            out[own[u] - N + v0] = Pack<T>::put(allowed[u] ? y : -INFINITY);
-        }
+        out[t] = Pack<T>::put(allowed ? y : -INFINITY);
     }
 }
 
@@ -269,7 +257,7 @@ int launch_adjust(const AdjustLogitsArgs& a, cudaStream_t stream) {
     AdjParams p = {a.logits, a.ld, a.out, a.ldo, (const long long*)a.tokens, a.ldk, a.lengths, a.prompt_lengths, a.repetition, a.presence, a.frequency, (const long long*)a.bias_ids, a.bias,
                    a.ldb, a.mask, a.ldm, a.repetition_all, a.presence_all, a.frequency_all, a.V, a.max_tokens, a.n_bias, 0};
     // Segments of a row: as few as shared memory allows, since every one reads all of the row's tokens, unless SMs would have nothing to do; then as many as the last round of CTAs has room for
-    // (64 rows of 151936: 9 of 17408 in two rounds 14 us, 10 of 16384 in three 20 us).
+    // (64 rows of 151936 with 4096 tokens and 100 biases: 4 of 38912 in one round 15.5 us; with counts of 32 bits 9 of 17408 in two rounds 18.5, 10 of 16384 in three 20.5).
     const long long slots = 1024ll / kAdjThreads * sms_of_current_device();
     long long n = ((long long)a.V + kLargest - 1) / kLargest;
     const long long rounds = (a.rows * n + slots - 1) / slots, most = ((long long)a.V + 2047) / 2048;
@@ -292,7 +280,7 @@ int launch_adjust(const AdjustLogitsArgs& a, cudaStream_t stream) {
 }  // namespace
 
 int launch_adjust_logits(int dtype, const AdjustLogitsArgs& a, cudaStream_t stream) {
-    // Long histories, which every CTA of a row reads, are read by fewer CTAs of twice the threads (8 rows of 151936 with 30000 tokens 13.3 -> 11.1 us; 64 rows with 4096 tokens 18.7, 20.9 that way).
+    // Long histories, which every CTA of a row reads, are read by fewer CTAs of twice the threads (8 rows of 151936 with 30000 tokens 13.3 -> 10.8 us; 64 rows with 4096 tokens 15.5, 20.9 that way).
     if (a.lengths && a.max_tokens > kAdjShort) return dtype == 1 ? launch_adjust<float, 1024>(a, stream) : launch_adjust<__nv_bfloat16, 1024>(a, stream);
     return dtype == 1 ? launch_adjust<float, 512>(a, stream) : launch_adjust<__nv_bfloat16, 512>(a, stream);
 }

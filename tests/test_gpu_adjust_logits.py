@@ -58,6 +58,26 @@ def test_adjust(rows, V, n_tok, n_bias, mask, dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n_tok", [8191, 8192, 8193, 20000])
+def test_long_histories(n_tok, dtype):
+    """Both sides of the line between the two widths of counts, one row that says a single token all the time."""
+    import seq_ops as S
+    x, kw = _inputs(n_tok, 3, 50257, n_tok, 20, True, dtype)
+    kw["tokens"][1] = 50256
+    kw["lengths"][1], kw["prompt_lengths"][1] = n_tok, 3
+    kw["frequency"][1] = 2.0 ** -12
+    _check(S.adjust_logits(x, **kw), x, kw)
+
+
+@pytest.mark.parametrize("rows,V,n_bias", [(1, 1000003, 50), (300, 40970, 5), (150, 82000, 0), (2, 163841, 4096)])
+def test_vocabularies_of_many_segments(rows, V, n_bias):
+    import seq_ops as S
+    x, kw = _inputs(rows, rows, V, 100, n_bias, True, torch.bfloat16)
+    kw["tokens"][:, :4] = torch.tensor([0, V - 1, V // 2, 7], device="cuda")
+    _check(S.adjust_logits(x, **kw), x, kw)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 def test_layouts(dtype):
     """Pitched and shifted logits and results (whole rows off the 16-byte grid, both alike and not), pitched tokens and biases, one mask for all rows, numbers for all rows."""
     import seq_ops as S
