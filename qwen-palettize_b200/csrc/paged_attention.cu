@@ -124,50 +124,78 @@ paged_attn_kernel(const PagedParams p) {
     pdl_wait();
 
     // ---- the line, and where this warp begins on it: a request is items * (steps + kSwitch) long, one without tokens 0
-    auto steps_of = [&](int b) { return (tokens_of(p, p.lengths[b]) + TOK - 1) / TOK; };
-    const int per = (p.B + NW * 32 - 1) / (NW * 32), r0 = min(p.B, tid * per), r1 = min(p.B, r0 + per);
-    long long mine = 0;
-    bool empty = false;
-    for (int b = r0; b < r1; ++b) {
-        const int n = steps_of(b);
-        mine += n ? n + kSwitch : 0;
-        empty |= n == 0;
-    }
-    long long upto = mine;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const long long u = __shfl_up_sync(0xFFFFFFFFu, upto, o);
-        if (lane >= o) upto += u;
-    }
-    sm_first[tid] = upto - mine;
-    if (lane == 31) sm_sum[warp] = upto;
-    if (lane < 2) sm_meta[warp][lane].flags = 0;
-    empty = __syncthreads_or(empty);
-    // lane w: the sum of the warps ahead of w; lane NW: all
-    long long ahead = 0;
-#pragma unroll
-    for (int w = 0; w < NW; ++w) ahead += w < lane ? sm_sum[w] : 0;
-    const long long total = __shfl_sync(0xFFFFFFFFu, ahead, NW) * p.items;
-    // every warp's stretch, and who is at work: CTA c from the places c * NW * stretch on
+    auto size_of = [&](int len) { const int n = (len + TOK - 1) / TOK; return n ? n + kSwitch : 0; };
     const int W = ctas * NW;
-    const long long stretch = max(total <= 0x7FFFFFFF - W ? (long long)(((int)total + W - 1) / W) : (total + W - 1) / W, 1ll);
-    const long long begin = (cta * NW + warp) * stretch;
+    long long total, stretch;
+    auto cut = [&](long long sum) {                 // every warp's stretch; CTA c works from the places c * NW * stretch on
+        total = sum * p.items;
+        stretch = max(total <= 0x7FFFFFFF - W ? (long long)(((int)total + W - 1) / W) : (total + W - 1) / W, 1ll);
+    };
     Place<TOK> eye;
-    eye.left = (int)min(total - begin, stretch);
-    if (eye.left > 0) {
-        // the thread whose requests hold that place, then the request
-        const int group = __popc(__ballot_sync(0xFFFFFFFFu, lane < NW && ahead * p.items <= begin)) - 1;
-        const long long base = __shfl_sync(0xFFFFFFFFu, ahead, group);
-        const int who = group * 32 + __popc(__ballot_sync(0xFFFFFFFFu, (base + sm_first[group * 32 + lane]) * p.items <= begin)) - 1;
-        long long off = begin - (base + sm_first[who]) * p.items;
-        eye.b = who * per;
-        while (true) {
-            eye.open(p, p.lengths[eye.b]);
-            const long long size = eye.n ? (long long)(eye.n + kSwitch) * p.items : 0;
-            if (off < size) break;
-            off -= size;
-            ++eye.b;
+    bool empty = false;
+    long long off;
+    if (lane < 2) sm_meta[warp][lane].flags = 0;
+    if (p.B <= 32) {
+        // a lane a request, every warp for itself: one request of 2049 tokens, replayed, 8.4 us; by the sums below 9.0
+        const int len = lane < p.B ? tokens_of(p, p.lengths[lane]) : 0, size = size_of(len);
+        long long upto = size;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const long long u = __shfl_up_sync(0xFFFFFFFFu, upto, o);
+            if (lane >= o) upto += u;
         }
+        empty = __any_sync(0xFFFFFFFFu, lane < p.B && size == 0);
+        cut(__shfl_sync(0xFFFFFFFFu, upto, 31));
+        const long long begin = (cta * NW + warp) * stretch;
+        eye.left = (int)min(total - begin, stretch);
+        // the last request that begins there or ahead; of several, all but it are empty
+        const int who = __popc(__ballot_sync(0xFFFFFFFFu, (upto - size) * p.items <= begin)) - 1;
+        off = begin - __shfl_sync(0xFFFFFFFFu, upto - size, who) * p.items;
+        eye.b = who;
+        eye.len = __shfl_sync(0xFFFFFFFFu, len, who);
+        eye.n = (eye.len + TOK - 1) / TOK;
+        eye.ahead = __shfl_sync(0xFFFFFFFFu, len, (who + 1) & 31);
+    } else {
+        const int per = (p.B + NW * 32 - 1) / (NW * 32), r0 = min(p.B, tid * per), r1 = min(p.B, r0 + per);
+        long long mine = 0;
+        for (int b = r0; b < r1; ++b) {
+            const int size = size_of(tokens_of(p, p.lengths[b]));
+            mine += size;
+            empty |= size == 0;
+        }
+        long long upto = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const long long u = __shfl_up_sync(0xFFFFFFFFu, upto, o);
+            if (lane >= o) upto += u;
+        }
+        sm_first[tid] = upto - mine;
+        if (lane == 31) sm_sum[warp] = upto;
+        empty = __syncthreads_or(empty);
+        // lane w: the sum of the warps ahead of w; lane NW: all
+        long long ahead = 0;
+#pragma unroll
+        for (int w = 0; w < NW; ++w) ahead += w < lane ? sm_sum[w] : 0;
+        cut(__shfl_sync(0xFFFFFFFFu, ahead, NW));
+        const long long begin = (cta * NW + warp) * stretch;
+        eye.left = (int)min(total - begin, stretch);
+        if (eye.left > 0) {
+            // the thread whose requests hold that place, then the request
+            const int group = __popc(__ballot_sync(0xFFFFFFFFu, lane < NW && ahead * p.items <= begin)) - 1;
+            const long long base = __shfl_sync(0xFFFFFFFFu, ahead, group);
+            const int who = group * 32 + __popc(__ballot_sync(0xFFFFFFFFu, (base + sm_first[group * 32 + lane]) * p.items <= begin)) - 1;
+            off = begin - (base + sm_first[who]) * p.items;
+            eye.b = who * per;
+            while (true) {
+                eye.open(p, p.lengths[eye.b]);
+                const long long size = (long long)size_of(eye.len) * p.items;
+                if (off < size) break;
+                off -= size;
+                ++eye.b;
+            }
+        }
+    }
+    if (eye.left > 0) {
         const int one = eye.n + kSwitch;
         eye.item = off <= 0x7FFFFFFF ? (int)off / one : (int)(off / one);
         eye.t = (int)(off - (long long)eye.item * one);

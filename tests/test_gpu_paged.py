@@ -208,7 +208,7 @@ def test_attention_lengths(page, lengths):
 
 @pytest.mark.parametrize("hq,hk,d,page,B,T", [(32, 8, 128, 16, 70, 1500), (16, 16, 64, 64, 200, 700), (8, 2, 256, 32, 40, 3000), (40, 2, 128, 16, 60, 5000), (4, 1, 128, 16, 1, 600000), (9, 3, 64, 128, 2000, 300)])
 def test_attention_with_many_steps(hq, hk, d, page, B, T):
-    """Enough work for it to be taken as it comes: right, and the same bits whoever takes it."""
+    """Enough work for many steps in every warp: right, and the same bits each time."""
     import plz_ops as ops
     g = torch.Generator().manual_seed(B)
     lengths = torch.randint(T // 2, T + 1, (B,), generator=g).tolist()
@@ -223,6 +223,27 @@ def test_attention_with_many_steps(hq, hk, d, page, B, T):
     check_status()
     _close(got[0], *ref.attention(*a, hq, hk, d))
     assert all(torch.equal(got[0], x) for x in got[1:])
+
+
+@pytest.mark.parametrize("B", [2, 31, 32, 33, 64])
+@pytest.mark.parametrize("hq,hk,d", [(8, 2, 128), (20, 1, 64), (4, 4, 256)])
+@pytest.mark.parametrize("holes", ["none", "ends", "inside", "most"])
+def test_attention_around_a_warp_of_requests(B, hq, hk, d, holes):
+    """Up to 32 requests a warp holds every length itself, above the CTA shares them; requests without tokens first, last and in runs."""
+    import plz_ops as ops
+    g = torch.Generator().manual_seed(B)
+    lengths = torch.randint(1, 400, (B,), generator=g)
+    if holes == "ends":
+        lengths[:B // 3] = lengths[B - B // 3:] = 0
+    elif holes == "inside":
+        lengths[1:B - 1] = 0
+    elif holes == "most":
+        lengths[torch.rand(B, generator=g) < 0.8] = 0
+    a = _case(B * d, lengths.tolist(), hq, hk, d, 16)
+    got = ops.attention_decode_paged(*a, hq, hk, d)
+    check_status()
+    _close(got, *ref.attention(*a, hq, hk, d))
+    assert (got[lengths == 0] == 0).all()
 
 
 @pytest.mark.parametrize("scale", [1.0, 0.02, -0.3, 0.0])
