@@ -626,7 +626,7 @@ int32_t plz_sample(const float* logits, int64_t ld, int32_t rows, int32_t V, flo
  *   is left out of the softmax and a length past `width` pages is cut, either of them (and a negative length) stores 1 to *bad (device int32, may be NULL); values are finite.
  *   ws: plz_attn_decode_paged_ws_bytes, 16-byte aligned, for any B and lengths; calls that may run at the same time need one each. Bits repeat from run to run; a request's may change with the other requests'
  *   lengths, which move the places where its sums are cut.
- * plz_adjust_logits: out = logits [rows, V] (dtype 0 bf16, 1 fp32, computed in fp32, out may be logits) after, in this order,
+ * plz_adjust_logits: out = logits [rows, V] (dtype 0 bf16, 1 fp32, computed in fp32, out may be logits with the same pitch) after, in this order,
  *   repetition r: x > 0 ? x / r : x * r for every token among tokens[0 .. lengths[row]) (int64 [rows, >= lengths], rows ldk apart);
  *   frequency f, presence p: x - f * c - p for tokens that occur c > 0 times among tokens[prompt_lengths[row] .. lengths[row]);
  *   bias: x + the biases of the token, fp32 bias[row, i] for token bias_ids[row, i], in the order of i;

@@ -1283,6 +1283,7 @@ int32_t plz_adjust_logits(int32_t dtype, const plz_adjust_logits_t* a, void* str
     if (!a->logits || !a->out || (a->lengths && a->max_tokens > 0 && !a->tokens) || (a->n_bias > 0 && (!a->bias_ids || !a->bias))) { set_last_error("null pointer"); return PLZ_ERR_NULL; }
     const uintptr_t size = dtype == 1 ? 4 : 2;
     if (((uintptr_t)a->logits | (uintptr_t)a->out) & (size - 1)) { set_last_error("adjust_logits: misaligned logits"); return PLZ_ERR_BAD_ALIGN; }
+    if (a->logits == a->out && a->rows > 1 && a->ld != a->ldo) { set_last_error("adjust_logits: in place, but rows of out lie elsewhere"); return PLZ_ERR_UNSUPPORTED; }
     return launch_adjust_logits(dtype, *a, (cudaStream_t)stream);
 }
 

@@ -84,6 +84,15 @@ def test_adjust_logits_refusals(built_lib):
     assert call(logits=PTR + 2) == ALIGN
 
 
+def test_adjust_logits_in_place_with_two_pitches(built_lib):
+    """Over the logits themselves, but with rows that lie elsewhere: a row's results would go over another row's logits."""
+    import plz_native as P
+    base = dict(logits=PTR, ld=100, out=PTR, ldo=104, tokens=None, ldk=0, lengths=None, prompt_lengths=None, repetition=None, presence=None, frequency=None, bias_ids=None, bias=None, ldb=0, mask=None,
+                ldm=0, repetition_all=1.0, presence_all=0.0, frequency_all=0.0, rows=2, V=100, max_tokens=0, n_bias=0)
+    call = _call(P.lib().plz_adjust_logits, P.AdjustLogits, base, lead=(1,))
+    assert call(rows=0) == OK and call() == UNSUPPORTED and call(ld=104, ldo=100) == UNSUPPORTED
+
+
 def test_binding_refusals(built_lib):
     """Types and shapes that the binding passes as bare pointers, and tensors that are not on a GPU."""
     import plz_native as P
