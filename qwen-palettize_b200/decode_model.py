@@ -91,7 +91,7 @@ class PagedKVCache:
         new[requests] = n
         p = self.plan(new.to(self.lengths.device), n * len(requests))
         for li in range(self.k.shape[0]):
-            k, v = (t[li, :, :n].reshape(n * len(requests), -1) for t in (cache.k, cache.v))
+            k, v = (t[li, :, :n].reshape(n * len(requests), t.shape[-1]) for t in (cache.k, cache.v))
             ops.write_pages(k, v, p.slots, self.k[li], self.v[li])
         return p
 

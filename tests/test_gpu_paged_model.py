@@ -155,6 +155,14 @@ def test_settings_of_a_request_in_the_engine():
         eng.generate([prompt], SamplingParams(allowed=lambda out: []))
 
 
+def test_an_empty_cache_fills_nothing():
+    m = _model(1)
+    c = m.new_paged_cache(2, 10, 16, 64)
+    p = c.fill(m.new_cache(2, 64), [0, 1])
+    assert p.status.tolist() == [0, 0] and p.slots.numel() == 0 and c.lengths.tolist() == [0, 0] and c.n_free.item() == 10
+    check_status()
+
+
 def test_settings_from_the_command_line(tmp_path, capsys):
     import cli
     import model_registry as R
