@@ -83,6 +83,8 @@ class Engine:
             raise ValueError("the repetition penalty is a positive factor")
         if any(not 0 <= t < self.model.vocab for t, _ in params.bias):
             raise ValueError(f"a bias for a token outside the vocabulary of {self.model.vocab}")
+        if len(params.bias) > 4096:
+            raise ValueError(f"{len(params.bias)} biases, at most 4096")
         if len(prompt) + params.max_new > self.pool.capacity:
             raise ValueError(f"{len(prompt)} + {params.max_new} tokens exceed the capacity {self.pool.capacity}")
         rid = ("gen", self._next)

@@ -163,6 +163,16 @@ def test_an_empty_cache_fills_nothing():
     check_status()
 
 
+def test_too_many_biases_are_refused_when_they_come():
+    from engine import Engine, SamplingParams
+    eng = Engine(_model(3), 64)
+    with pytest.raises(ValueError):
+        eng.submit([5, 17], SamplingParams(bias=((1, 0.5),) * 4097))
+    assert not eng.waiting
+    out = eng.generate([[5, 17]], SamplingParams(max_new=2, bias=((7, 0.125),) * 4096))[0]      # 512 in all
+    assert out == [7, 7]
+
+
 def test_settings_from_the_command_line(tmp_path, capsys):
     import cli
     import model_registry as R
