@@ -114,7 +114,12 @@ class Engine:
         else:
             logits = self.step(r.rid, [r.out[-1]], [0])
         if logits is not None and r.params.max_new > 0:
-            self._take(r, logits)
+            try:
+                self._take(r, logits)
+            except Exception:            # its settings failed: it ends, the others go on with the next call
+                self.live.remove(r)
+                self.end(r.rid)
+                raise
         if r.done or (r.fed == len(r.prompt) and len(r.out) >= r.params.max_new):
             self.live.remove(r)
             self.end(r.rid)

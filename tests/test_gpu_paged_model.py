@@ -173,6 +173,19 @@ def test_too_many_biases_are_refused_when_they_come():
     assert out == [7, 7]
 
 
+def test_a_request_that_fails_ends_alone():
+    """No token allowed at the third: the request is gone, the other one gives what it gives by itself."""
+    from engine import Engine, SamplingParams
+    m = _model(3)
+    want = Engine(m, 64).generate([[9, 4, 2]], SamplingParams(max_new=6))[0]
+    eng = Engine(m, 64)
+    bad = eng.submit([5, 17], SamplingParams(max_new=6, allowed=lambda out: range(1000) if len(out) < 2 else []))
+    good = eng.submit([9, 4, 2], SamplingParams(max_new=6))
+    with pytest.raises(ValueError):
+        eng.run()
+    assert eng.run()[good] == want and bad not in eng.finished and bad not in eng.pool
+
+
 def test_settings_from_the_command_line(tmp_path, capsys):
     import cli
     import model_registry as R
