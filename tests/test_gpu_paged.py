@@ -316,6 +316,32 @@ def test_pages_and_lengths_that_do_not_exist():
     assert got[2].isnan().all()
 
 
+@pytest.mark.parametrize("hq,hk,d", [(8, 1, 128), (4, 2, 64), (4, 1, 256), (9, 1, 128), (16, 1, 64), (17, 1, 256)])
+def test_weights_enter_the_product_with_all_their_bits(hq, hk, d):
+    """A weight w = e^s against tokens of weight 1 whose values are -w in three bf16 terms: what is left is the weight's own error. Off by 2^-23 w through the exponent (two roundings of 2^-24 of
+    |s| log2(e) <= 1.45, times ln 2), 2^-22 w through the exponential, and by four sums below 2 that may drop 2^-24 of it each (all other products are multiples of 2^-24): 2^-21 in all. Two bf16 terms
+    of w would leave up to 2^-18."""
+    import plz_ops as ops
+    s = -torch.arange(1, 201).double().div(256).bfloat16().double()      # scores, exact in bf16
+    w, B = s.exp(), s.numel()
+    terms, left = [], w.clone()
+    for _ in range(3):
+        terms.append(left.bfloat16().double())
+        left = left - terms[-1]
+    kp, vp = (torch.zeros(B, 4, hk * d, dtype=torch.float64) for _ in range(2))
+    kp[:, 0, ::d] = s[:, None]
+    vp[:, 0] = 1.0
+    for i, t in enumerate(terms):
+        vp[:, 1 + i] = -t[:, None]
+    q = torch.zeros(B, hq * d, dtype=torch.bfloat16, device="cuda")
+    q[:, ::d] = 1.0
+    kp, vp = (t.bfloat16().cuda() for t in (kp, vp))
+    got = ops.attention_decode_paged(q, kp, vp, torch.arange(B, dtype=I32, device="cuda")[:, None].contiguous(), torch.full((B,), 4, dtype=I32, device="cuda"), hq, hk, d, scale=1.0)
+    got, w = got.double().cpu(), w[:, None]
+    bound = (1.5 * 2.0 ** -22 * w + 4 * 2.0 ** -23 + left.abs()[:, None]) / (3 + w) * (1 + 2.0 ** -8)
+    assert (got.abs() <= bound).all(), float((got.abs() / bound).max())
+
+
 def test_attention_repeats_bit_for_bit_and_on_another_stream():
     import plz_ops as ops
     a = _case(1, RAGGED * 3, 32, 8, 128, 16)
