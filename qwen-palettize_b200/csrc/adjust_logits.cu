@@ -53,12 +53,12 @@ template <> struct Pack<__nv_bfloat16> {
     __device__ __forceinline__ static uint4 masked(const uint4& v, uint32_t bits) { return make_uint4(two(v.x, bits), two(v.y, bits >> 2), two(v.z, bits >> 4), two(v.w, bits >> 6)); }
 };
 
-struct RowSettings { float r, inv, p, f; };      // inv = 1 / r: x * inv is within 2^-23 of x / r
+struct RowSettings { float r, p, f; };
 
 template <typename M>
 __device__ __forceinline__ float penalized(float x, uint32_t n, const RowSettings& s) {
     const uint32_t c = n & M::kCount;
-    if (n & (M::kSeen | M::kCount)) x *= x > 0.f ? s.inv : s.r;
+    if (n & (M::kSeen | M::kCount)) x = x > 0.f ? x / s.r : x * s.r;
     return c ? x - s.f * (float)c - s.p : x;
 }
 
@@ -194,7 +194,6 @@ adjust_logits_kernel(const AdjParams p) {
     if (!marks) return;
     RowSettings s;
     s.r = p.repetition ? p.repetition[row] : p.repetition_all;
-    s.inv = 1.f / s.r;
     s.p = p.presence ? p.presence[row] : p.presence_all;
     s.f = p.frequency ? p.frequency[row] : p.frequency_all;
     __syncthreads();

@@ -115,6 +115,21 @@ def test_logits_that_are_no_numbers_stay_so():
     assert got[0] == float("inf") and got[1] == float("-inf") and got[2] != got[2] and got[3] == -0.5 and got[4] == -1.0
 
 
+def test_repetition_is_one_rounded_operation():
+    """x / r and x * r as fp32 makes them, to the last bit, for factors whose inverse has no fp32 value too."""
+    import seq_ops as S
+    factors = [1.1, 1.3, 1.7, 3.0, 0.7, 1e-39, 2.0 ** -149, 3e38, 1e30]
+    V = 4099
+    g = torch.Generator(device="cuda").manual_seed(4)
+    x = torch.randn(len(factors), V, generator=g, device="cuda") * torch.tensor([1, 1, 1, 1, 1, 1e-3, 1e-10, 1e30, 1e30], device="cuda")[:, None]
+    r = torch.tensor(factors, device="cuda")
+    tok = torch.arange(V, device="cuda").expand(len(factors), -1)
+    got = S.adjust_logits(x, tokens=tok, lengths=torch.full((len(factors),), V, dtype=torch.int32, device="cuda"), repetition=r)
+    x, r = x.cpu(), r.cpu()[:, None]
+    want = torch.where(x > 0, x / r, x * r)
+    assert torch.isfinite(want[5]).all() and torch.equal(got.cpu(), want)
+
+
 def test_a_token_said_very_often_and_every_token_biased():
     import seq_ops as S
     V, n = 700, 100000
