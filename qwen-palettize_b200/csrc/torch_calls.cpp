@@ -299,18 +299,8 @@ PyObject* plan_pages(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const at::Tensor* add = numbers(a[1], B);
     if (!add || !(tab = rows_like(a[2], at::kInt, B))) Py_RETURN_NONE;
     if ((a[8] != Py_None && !(len_out = numbers(a[8], B))) || (a[9] != Py_None && !(count_out = numbers(a[9], 1)))) Py_RETURN_NONE;
-    // one piece of memory for all that is new: an allocation costs more than the kernel of a small step
-    const int64_t size[6] = {len_out ? 0 : B, count_out ? 0 : 1, B + 1, rows, rows, B};
-    int64_t at[6], all = 0;
-    for (int i = 0; i < 6; ++i) { at[i] = all; all += (size[i] + 3) / 4 * 4; }
-    const at::Tensor room = result(*len, {all}, at::kInt);
-    auto part = [&](int i) {
-        at::Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(room.storage()), room.key_set(), room.dtype());
-        t.unsafeGetTensorImpl()->set_storage_offset(at[i]);
-        t.unsafeGetTensorImpl()->set_sizes_contiguous({size[i]});
-        return t;
-    };
-    at::Tensor out[6] = {len_out ? *len_out : part(0), count_out ? *count_out : part(1), part(2), part(3), part(4), part(5)};
+    auto part = [&](int64_t size) { return result(*len, {size}, at::kInt); };      // storages of their own: a caller may keep, save or resize one of them
+    at::Tensor out[6] = {len_out ? *len_out : part(B), count_out ? *count_out : part(1), part(B + 1), part(rows), part(rows), part(B)};
     int32_t* o[6];
     for (int i = 0; i < 6; ++i) o[i] = (int32_t*)out[i].data_ptr();
     const plz_page_plan_t p = {(const int32_t*)len->data_ptr(), (const int32_t*)add->data_ptr(), (int32_t*)tab->data_ptr(), tab->stride(0), (int32_t*)stack->data_ptr(),

@@ -450,6 +450,18 @@ def test_general_path_and_native_calls_agree(monkeypatch):
         everything()
 
 
+def test_results_of_a_plan_have_storages_of_their_own():
+    """Growing one of them leaves the others as they are, and saving one saves no more than it."""
+    import plz_ops as ops
+    p = ops.plan_pages(_dev([3, 0]), _dev([2, 5]), _dev([[4, -1], [-1, -1]]), _dev([0, 1, 2, 3, -1]), _dev([4]), 4, 8)
+    parts = (p.lengths, p.n_free, p.starts, p.slots, p.positions, p.status)
+    assert len({t.untyped_storage().data_ptr() for t in parts}) == 6
+    assert all(t.storage_offset() == 0 and t.untyped_storage().nbytes() == 4 * t.numel() for t in parts)
+    positions = p.positions.clone()
+    p.slots.resize_(16).fill_(99)
+    assert torch.equal(p.positions, positions)
+
+
 def test_results_that_are_written_past_are_refused():
     import plz_native as P
     import plz_ops as ops
