@@ -1219,7 +1219,9 @@ int32_t plz_page_plan(const plz_page_plan_t* a, void* stream) {
     if (a->B > 16384 || (int64_t)a->B * a->width >= (1 << 30) || (int64_t)a->n_pages * a->page_size > 0x7FFFFFFF || a->max_rows > (1 << 30)) {
         set_last_error("page_plan: more than 16384 requests, 2^30 table entries or rows, or 2^31 slots"); return PLZ_ERR_TOO_LARGE;
     }
-    if (a->B > 0 && a->lengths == a->new_tokens) { set_last_error("page_plan: the lengths may not go where the new tokens are"); return PLZ_ERR_UNSUPPORTED; }
+    if (a->B > 0 && (a->lengths == a->new_tokens || a->status == a->new_tokens || a->status == a->cached || a->status == a->lengths)) {
+        set_last_error("page_plan: the lengths may not go where the new tokens are, the status where either is"); return PLZ_ERR_UNSUPPORTED;
+    }
     return launch_page_plan(*a, (cudaStream_t)stream);
 }
 

@@ -288,19 +288,19 @@ bool pools(PyObject* ko, PyObject* vo, int64_t cols, const at::Tensor*& k, const
     return k->sizes() == v->sizes() && k->strides() == v->strides() && k->size(0) <= 0x7FFFFFFF && k->size(1) <= 0x7FFFFFFF;
 }
 
-// (lengths, new_tokens, table, free_pages, n_free, page_size, max_rows, row_pitch, lengths_out or None, n_free_out or None) -> (lengths, n_free, starts, slots, positions, status)
+// (lengths, new_tokens, table, free_pages, n_free, page_size, max_rows, row_pitch, lengths_out or None, n_free_out or None, status_out or None) -> (lengths, n_free, starts, slots, positions, status)
 PyObject* plan_pages(PyObject*, PyObject* const* a, Py_ssize_t n) {
     HANDLE_TH_ERRORS
-    if (n != 10) Py_RETURN_NONE;
-    const at::Tensor *len = numbers(a[0]), *stack = numbers(a[3]), *count = numbers(a[4], 1), *tab, *len_out = nullptr, *count_out = nullptr;
+    if (n != 11) Py_RETURN_NONE;
+    const at::Tensor *len = numbers(a[0]), *stack = numbers(a[3]), *count = numbers(a[4], 1), *tab, *len_out = nullptr, *count_out = nullptr, *status_out = nullptr;
     int64_t page, rows, pitch;
     if (!len || !stack || !count || len->size(0) > 0x7FFFFFFF || stack->size(0) > 0x7FFFFFFF || !small(a[5], page) || !small(a[6], rows) || !small(a[7], pitch)) Py_RETURN_NONE;
     const int64_t B = len->size(0);
     const at::Tensor* add = numbers(a[1], B);
     if (!add || !(tab = rows_like(a[2], at::kInt, B))) Py_RETURN_NONE;
-    if ((a[8] != Py_None && !(len_out = numbers(a[8], B))) || (a[9] != Py_None && !(count_out = numbers(a[9], 1)))) Py_RETURN_NONE;
+    if ((a[8] != Py_None && !(len_out = numbers(a[8], B))) || (a[9] != Py_None && !(count_out = numbers(a[9], 1))) || (a[10] != Py_None && !(status_out = numbers(a[10], B)))) Py_RETURN_NONE;
     auto part = [&](int64_t size) { return result(*len, {size}, at::kInt); };      // storages of their own: a caller may keep, save or resize one of them
-    at::Tensor out[6] = {len_out ? *len_out : part(B), count_out ? *count_out : part(1), part(B + 1), part(rows), part(rows), part(B)};
+    at::Tensor out[6] = {len_out ? *len_out : part(B), count_out ? *count_out : part(1), part(B + 1), part(rows), part(rows), status_out ? *status_out : part(B)};
     int32_t* o[6];
     for (int i = 0; i < 6; ++i) o[i] = (int32_t*)out[i].data_ptr();
     const plz_page_plan_t p = {(const int32_t*)len->data_ptr(), (const int32_t*)add->data_ptr(), (int32_t*)tab->data_ptr(), tab->stride(0), (int32_t*)stack->data_ptr(),

@@ -65,6 +65,7 @@ class PagedKVCache:
         self.lengths = torch.zeros(B, dtype=torch.int32, device=device)
         self.free_pages = torch.arange(n_pages, dtype=torch.int32, device=device)
         self.n_free = torch.full((1,), n_pages, dtype=torch.int32, device=device)
+        self.status = torch.zeros(B, dtype=torch.int32, device=device)        # of the last plan, replayed ones too: 0 done, 1 out of pages, 2 does not fit
 
     @property
     def requests(self) -> int:
@@ -77,8 +78,9 @@ class PagedKVCache:
 
     def plan(self, new_tokens: torch.Tensor, max_rows: int, row_pitch: int = 0) -> ops.PagePlan:
         """Pages for the next tokens of every request (int32 [B] on the device; 0: none, negative: the request has ended and gives its pages back); the lengths
-        of the cache are those afterwards. May be captured."""
-        return ops.plan_pages(self.lengths, new_tokens, self.table, self.free_pages, self.n_free, self.page_size, max_rows, row_pitch, lengths_out=self.lengths, n_free_out=self.n_free)
+        and the status of the cache are those afterwards. May be captured."""
+        return ops.plan_pages(self.lengths, new_tokens, self.table, self.free_pages, self.n_free, self.page_size, max_rows, row_pitch, lengths_out=self.lengths, n_free_out=self.n_free,
+                              status_out=self.status)
 
     def fill(self, cache: KVCache, requests) -> ops.PagePlan:
         """The filled positions of `cache`, one sequence for each of `requests` (row numbers in increasing order) that hold nothing yet: prompts' keys and values after prefill. The plan's
@@ -269,7 +271,8 @@ class PalettizedQwen:
 
     def decode_paged(self, ids: torch.Tensor, cache: PagedKVCache, new_tokens: torch.Tensor) -> torch.Tensor:
         """One token for every request of `cache` with new_tokens[b] = 1 (int32 [B] on the device; 0: none, negative: ended): ids int64 [B] -> logits bf16 [B, vocab] of the tokens after
-        them. Rows of requests without a token, or without a page for it (the plan's status), hold nothing of use. Nothing waits for the device, so a step can be captured."""
+        them. cache.status[b] is not 0 for a request whose token found no page (1) or does not fit (2): it keeps its length, and the token can be brought again. Its row, and those of requests
+        without a token, hold nothing of use. Nothing waits for the device, so a step can be captured."""
         c = self.cfg
         B = cache.requests
         if cache.capacity > self.cos.shape[0]:

@@ -94,6 +94,45 @@ def test_more_tokens_than_the_model_has_positions_are_refused():
             c.fill(m.new_cache(2, 128), rows)
 
 
+@pytest.mark.parametrize("captured", [False, True])
+def test_a_step_without_a_page_for_a_request_is_told(captured):
+    """Three requests, pages for two: who got none is told by the cache's status, keeps its length, and goes on as if nothing had been once another one has ended."""
+    m = _model(4)
+    B, page = 3, 4
+    cache = m.new_paged_cache(B, n_pages=4, page_size=page, max_tokens=64)
+    alone = [m.new_cache(1, 64) for _ in range(B)]
+    ids, new = torch.zeros(B, dtype=torch.int64, device="cuda"), torch.zeros(B, dtype=torch.int32, device="cuda")
+    status = cache.status
+    step = lambda: m.decode_paged(ids, cache, new)
+    if captured:
+        step()
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = step()
+        step = lambda: (graph.replay(), out)[1]
+    g = torch.Generator().manual_seed(6)
+    tokens = torch.randint(0, 1000, (B, 20), generator=g).tolist()
+    at, seen = [0] * B, []
+    for t in range(10):
+        bring = [-1 if t == 7 else int(t < 7), 1, 1]
+        ids.copy_(torch.tensor([tokens[b][at[b]] for b in range(B)]))
+        new.copy_(torch.tensor(bring, dtype=torch.int32))
+        got = step()
+        told = status.tolist()
+        seen.append(told)
+        for b in range(B):
+            if bring[b] < 0:
+                alone[b].reset()
+                at[b] = 0
+            elif bring[b] and told[b] == 0:
+                assert_close(got[b:b + 1], m.decode_step(torch.tensor([tokens[b][at[b]]], device="cuda"), alone[b]), "logits", rel=3e-2, cos=0.999)
+                at[b] += 1
+        assert cache.lengths.tolist() == at and cache.status is status
+    # four pages: one each for the first four tokens, one for request 0's fifth; the others wait until it has ended and gave two back
+    assert seen == [[0, 0, 0]] * 4 + [[0, 1, 1]] * 4 + [[0, 0, 0]] * 2 and at == [0, 6, 6]
+
+
 def test_a_step_of_a_batch_together():
     """Plan, decode, settings, sampling: the step of a server, for requests that each have settings of their own, against the plain formulas on the same logits."""
     import paged_cases as ref
