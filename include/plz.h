@@ -613,7 +613,7 @@ int32_t plz_sample(const float* logits, int64_t ld, int32_t rows, int32_t V, flo
  *   a negative number ends it: its pages go back, its length becomes 0. Free pages are free_pages[0 .. *n_free), taken from the end by the requests in order;
  *   what ended requests give back is on top afterwards, in their order, and serves the next step.
  *   status[b] (int32 [B]): 0 done; 1 the free pages do not suffice for it (nor for any later request that needs one); 2 it does not fit: cached[b] < 0, more tokens than `width`
- *   pages or 2^31 - 1 hold, rows past max_rows or more than row_pitch. A request with status 1 or 2 keeps its pages and its length.
+ *   pages, max_tokens (0: no such limit) or 2^31 - 1 hold, rows past max_rows or more than row_pitch. A request with status 1 or 2 keeps its pages and its length.
  *   starts (int32 [B + 1]): first row of each request among the step's token rows: the running sum of the new tokens, or b * row_pitch where row_pitch > 0.
  *   slots, positions (int32 [max_rows]): page * page_size + row in the page, and position, of every token row; -1 for rows of nobody or of a request with status 1 or 2.
  *   lengths (int32 [B]), n_free_out: afterwards; may be `cached` and `n_free` themselves, nothing else may overlap. table gets the new pages.
@@ -639,7 +639,7 @@ typedef struct plz_page_plan {
     int32_t* free_pages; const int32_t* n_free;
     int32_t* lengths; int32_t* n_free_out;
     int32_t* starts; int32_t* slots; int32_t* positions; int32_t* status;
-    int32_t B, width, page_size, n_pages, max_rows, row_pitch;
+    int32_t B, width, page_size, n_pages, max_rows, row_pitch, max_tokens;
 } plz_page_plan_t;
 int32_t plz_page_plan(const plz_page_plan_t* args, void* stream);
 typedef struct plz_page_write {

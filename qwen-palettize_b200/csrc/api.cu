@@ -1213,8 +1213,8 @@ int32_t plz_sample(const float* logits, int64_t ld, int32_t rows, int32_t V, flo
 int32_t plz_page_plan(const plz_page_plan_t* a, void* stream) {
     if (!a || !a->n_free || !a->n_free_out || !a->starts || (a->B > 0 && (!a->cached || !a->new_tokens || !a->lengths || !a->status || (a->width > 0 && !a->table))) ||
         (a->n_pages > 0 && !a->free_pages) || (a->max_rows > 0 && (!a->slots || !a->positions))) { set_last_error("null pointer"); return PLZ_ERR_NULL; }
-    if (a->B < 0 || a->width < 0 || a->page_size <= 0 || a->n_pages < 0 || a->max_rows < 0 || a->row_pitch < 0 || (a->B > 1 && a->ldt < a->width)) {
-        set_last_error("page_plan: bad shape B=%d width=%d page=%d pages=%d rows=%d pitch=%d", a->B, a->width, a->page_size, a->n_pages, a->max_rows, a->row_pitch); return PLZ_ERR_BAD_SHAPE;
+    if (a->B < 0 || a->width < 0 || a->page_size <= 0 || a->n_pages < 0 || a->max_rows < 0 || a->row_pitch < 0 || a->max_tokens < 0 || (a->B > 1 && a->ldt < a->width)) {
+        set_last_error("page_plan: bad shape B=%d width=%d page=%d pages=%d rows=%d pitch=%d tokens=%d", a->B, a->width, a->page_size, a->n_pages, a->max_rows, a->row_pitch, a->max_tokens); return PLZ_ERR_BAD_SHAPE;
     }
     if (a->B > 16384 || (int64_t)a->B * a->width >= (1 << 30) || (int64_t)a->n_pages * a->page_size > 0x7FFFFFFF || a->max_rows > (1 << 30)) {
         set_last_error("page_plan: more than 16384 requests, 2^30 table entries or rows, or 2^31 slots"); return PLZ_ERR_TOO_LARGE;

@@ -52,7 +52,7 @@ page_plan_kernel(const PagePlanArgs a) {
     int *start = sm, *base = start + a.B + 1, *have = base + a.B;      // first row, stack index of page 0 (page j is below it by j), cached tokens
     const int tid = threadIdx.x, cta = blockIdx.x, ctas = gridDim.x;
     const int per = (a.B + kPlanThreads - 1) / kPlanThreads, b0 = min(a.B, tid * per), b1 = min(a.B, b0 + per);
-    const long long room = min((long long)a.width * a.page_size, (long long)INT32_MAX);
+    const long long room = min((long long)a.width * a.page_size, (long long)(a.max_tokens ? a.max_tokens : INT32_MAX));
     const Pages pages = {a.page_size, (a.page_size & (a.page_size - 1)) == 0 ? __ffs(a.page_size) - 1 : -1};
     if (tid == 0) sm_taken = 0;
     pdl_launch_dependents();

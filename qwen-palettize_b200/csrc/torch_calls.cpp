@@ -288,13 +288,13 @@ bool pools(PyObject* ko, PyObject* vo, int64_t cols, const at::Tensor*& k, const
     return k->sizes() == v->sizes() && k->strides() == v->strides() && k->size(0) <= 0x7FFFFFFF && k->size(1) <= 0x7FFFFFFF;
 }
 
-// (lengths, new_tokens, table, free_pages, n_free, page_size, max_rows, row_pitch, lengths_out or None, n_free_out or None, status_out or None) -> (lengths, n_free, starts, slots, positions, status)
+// (lengths, new_tokens, table, free_pages, n_free, page_size, max_rows, row_pitch, lengths_out or None, n_free_out or None, status_out or None, max_tokens) -> (lengths, n_free, starts, slots, positions, status)
 PyObject* plan_pages(PyObject*, PyObject* const* a, Py_ssize_t n) {
     HANDLE_TH_ERRORS
-    if (n != 11) Py_RETURN_NONE;
+    if (n != 12) Py_RETURN_NONE;
     const at::Tensor *len = numbers(a[0]), *stack = numbers(a[3]), *count = numbers(a[4], 1), *tab, *len_out = nullptr, *count_out = nullptr, *status_out = nullptr;
-    int64_t page, rows, pitch;
-    if (!len || !stack || !count || len->size(0) > 0x7FFFFFFF || stack->size(0) > 0x7FFFFFFF || !small(a[5], page) || !small(a[6], rows) || !small(a[7], pitch)) Py_RETURN_NONE;
+    int64_t page, rows, pitch, most;
+    if (!len || !stack || !count || len->size(0) > 0x7FFFFFFF || stack->size(0) > 0x7FFFFFFF || !small(a[5], page) || !small(a[6], rows) || !small(a[7], pitch) || !small(a[11], most)) Py_RETURN_NONE;
     const int64_t B = len->size(0);
     const at::Tensor* add = numbers(a[1], B);
     if (!add || !(tab = rows_like(a[2], at::kInt, B))) Py_RETURN_NONE;
@@ -305,7 +305,7 @@ PyObject* plan_pages(PyObject*, PyObject* const* a, Py_ssize_t n) {
     for (int i = 0; i < 6; ++i) o[i] = (int32_t*)out[i].data_ptr();
     const plz_page_plan_t p = {(const int32_t*)len->data_ptr(), (const int32_t*)add->data_ptr(), (int32_t*)tab->data_ptr(), tab->stride(0), (int32_t*)stack->data_ptr(),
                                (const int32_t*)count->data_ptr(), o[0], o[1], o[2], o[3], o[4], o[5], (int32_t)B, (int32_t)tab->size(1), (int32_t)page, (int32_t)stack->size(0),
-                               (int32_t)rows, (int32_t)pitch};
+                               (int32_t)rows, (int32_t)pitch, (int32_t)most};
     if (!launch([&](void* s) { return plz_page_plan(&p, s); })) Py_RETURN_NONE;
     PyObject* t = PyTuple_New(6);
     if (!t) return nullptr;

@@ -57,7 +57,9 @@ class PagedKVCache:
     """Keys and values of up to B requests of different lengths, in pages that the device hands out from one pool. A request keeps its row b of the table until it is ended."""
 
     def __init__(self, n_layers: int, B: int, n_pages: int, page_size: int, max_tokens: int, width: int, device):
-        self.page_size = page_size
+        if page_size < 1 or max_tokens < 0:
+            raise ValueError(f"pages of {page_size} and requests of {max_tokens} tokens")
+        self.page_size, self.max_tokens = page_size, max_tokens
         shape = (n_layers, n_pages, page_size, width)
         self.k = torch.empty(shape, dtype=torch.bfloat16, device=device)      # what no request has written is never read
         self.v = torch.empty(shape, dtype=torch.bfloat16, device=device)
@@ -74,13 +76,13 @@ class PagedKVCache:
     @property
     def capacity(self) -> int:
         """Most tokens of a request."""
-        return self.table.shape[1] * self.page_size
+        return self.max_tokens
 
     def plan(self, new_tokens: torch.Tensor, max_rows: int, row_pitch: int = 0) -> ops.PagePlan:
         """Pages for the next tokens of every request (int32 [B] on the device; 0: none, negative: the request has ended and gives its pages back); the lengths
         and the status of the cache are those afterwards. May be captured."""
         return ops.plan_pages(self.lengths, new_tokens, self.table, self.free_pages, self.n_free, self.page_size, max_rows, row_pitch, lengths_out=self.lengths, n_free_out=self.n_free,
-                              status_out=self.status)
+                              status_out=self.status, max_tokens=self.max_tokens)
 
     def fill(self, cache: KVCache, requests) -> ops.PagePlan:
         """The filled positions of `cache`, one sequence for each of `requests` (row numbers in increasing order) that hold nothing yet: prompts' keys and values after prefill. The plan's

@@ -117,7 +117,8 @@ class LatentAttn(C.Structure):
 class PagePlan(C.Structure):
     _fields_ = [("cached", C.c_void_p), ("new_tokens", C.c_void_p), ("table", C.c_void_p), ("ldt", C.c_int64), ("free_pages", C.c_void_p), ("n_free", C.c_void_p),
                 ("lengths", C.c_void_p), ("n_free_out", C.c_void_p), ("starts", C.c_void_p), ("slots", C.c_void_p), ("positions", C.c_void_p), ("status", C.c_void_p),
-                ("B", C.c_int32), ("width", C.c_int32), ("page_size", C.c_int32), ("n_pages", C.c_int32), ("max_rows", C.c_int32), ("row_pitch", C.c_int32)]
+                ("B", C.c_int32), ("width", C.c_int32), ("page_size", C.c_int32), ("n_pages", C.c_int32), ("max_rows", C.c_int32), ("row_pitch", C.c_int32),
+                ("max_tokens", C.c_int32)]
 
 
 class PageWrite(C.Structure):

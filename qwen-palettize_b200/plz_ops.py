@@ -646,13 +646,14 @@ def _int32(t: torch.Tensor, shape, what: str):
 
 
 def plan_pages(lengths: torch.Tensor, new_tokens: torch.Tensor, table: torch.Tensor, free_pages: torch.Tensor, n_free: torch.Tensor, page_size: int, max_rows: int,
-               row_pitch: int = 0, lengths_out: torch.Tensor | None = None, n_free_out: torch.Tensor | None = None, status_out: torch.Tensor | None = None) -> PagePlan:
+               row_pitch: int = 0, lengths_out: torch.Tensor | None = None, n_free_out: torch.Tensor | None = None, status_out: torch.Tensor | None = None,
+               max_tokens: int = 0) -> PagePlan:
     """Pages and slots of the next step of a batch of requests, without a look at the device's numbers from the host. lengths, new_tokens int32 [B]: cached tokens and tokens that
     the step brings, in order of the requests (row_pitch > 0: row_pitch rows for every request); a negative number ends the request and gives its pages back. table int32 [B, width] names
-    the requests' pages and gets the new ones; free_pages int32 [n_pages], whose first n_free (int32 [1]) entries are free, taken from the end. A request that the free pages or `width` pages do not
-    suffice for keeps what it has (status). lengths_out, n_free_out, status_out: where the new counts and the status go, `lengths` and `n_free` themselves for a step that is captured; None: new
+    the requests' pages and gets the new ones; free_pages int32 [n_pages], whose first n_free (int32 [1]) entries are free, taken from the end. A request that the free pages, `width` pages or
+    max_tokens tokens (0: no such limit) do not suffice for keeps what it has (status). lengths_out, n_free_out, status_out: where the new counts and the status go, `lengths` and `n_free` themselves for a step that is captured; None: new
     tensors."""
-    got = P.calls().plan_pages(lengths, new_tokens, table, free_pages, n_free, page_size, max_rows, row_pitch, lengths_out, n_free_out, status_out)
+    got = P.calls().plan_pages(lengths, new_tokens, table, free_pages, n_free, page_size, max_rows, row_pitch, lengths_out, n_free_out, status_out, max_tokens)
     if got is not None:
         return PagePlan(*got)
     B = lengths.shape[0]
@@ -665,7 +666,7 @@ def plan_pages(lengths: torch.Tensor, new_tokens: torch.Tensor, table: torch.Ten
     p = PagePlan(lengths_out if lengths_out is not None else new(B), n_free_out if n_free_out is not None else new(1), new(B + 1), new(max_rows), new(max_rows),
                  status_out if status_out is not None else new(B))
     a = P.PagePlan(lengths.data_ptr(), new_tokens.data_ptr(), table.data_ptr(), table.stride(0), free_pages.data_ptr(), n_free.data_ptr(), p.lengths.data_ptr(), p.n_free.data_ptr(),
-                   p.starts.data_ptr(), p.slots.data_ptr(), p.positions.data_ptr(), p.status.data_ptr(), B, table.shape[1], page_size, free_pages.shape[0], max_rows, row_pitch)
+                   p.starts.data_ptr(), p.slots.data_ptr(), p.positions.data_ptr(), p.status.data_ptr(), B, table.shape[1], page_size, free_pages.shape[0], max_rows, row_pitch, max_tokens)
     P.check(P.lib().plz_page_plan(C.byref(a), P.stream_ptr()), "plz_page_plan")
     return p
 

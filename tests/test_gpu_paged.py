@@ -78,6 +78,21 @@ def test_plan_of_a_padded_batch(pitch):
     _check_plan(*a, 16, 50 * pitch + 5, pitch=pitch)
 
 
+def test_plan_with_fewer_tokens_a_request_than_its_pages_hold():
+    import plz_ops as ops
+    cached, new = [5, 9, 10, 0, 11, 8, 10], [5, 2, 0, 11, -1, 2, -1]
+    table = torch.full((7, 3), -1, dtype=I32, device="cuda")
+    for b, n in enumerate(cached):
+        table[b, : -(-n // 4)] = _dev([b * 3 + j for j in range(-(-n // 4))])
+    want = [0, 2, 0, 2, 2, 0, 0]
+    for B in (7, 1000):                      # the small kernel and the large one
+        more = B - 7
+        p = ops.plan_pages(_dev(cached + [0] * more), _dev(new + [0] * more), torch.cat([table.clone(), torch.full((more, 3), -1, dtype=I32, device="cuda")]), _dev(list(range(30, 60))), _dev([30]),
+                           4, 30, max_tokens=10)
+        assert p.status.tolist() == want + [0] * more
+        assert p.lengths.tolist() == [10, 9, 10, 0, 11, 10, 0] + [0] * more
+
+
 def test_plan_of_nothing():
     import plz_ops as ops
     e = torch.zeros(0, dtype=I32, device="cuda")

@@ -133,6 +133,35 @@ def test_a_step_without_a_page_for_a_request_is_told(captured):
     assert seen == [[0, 0, 0]] * 4 + [[0, 1, 1]] * 4 + [[0, 0, 0]] * 2 and at == [0, 6, 6]
 
 
+@pytest.mark.parametrize("page_size", [16, 24, 100, 1000])
+def test_the_default_cache_serves_all_positions_and_no_more(page_size):
+    """Pages that do not divide the model's 512 positions: a request gets all of them, and the next token is refused although its last page has room."""
+    m = _model(1)
+    cache = m.new_paged_cache(2, n_pages=80, page_size=page_size)
+    assert cache.capacity == 512
+    kv = m.new_cache(1, 511)
+    kv.length = 511
+    assert cache.fill(kv, [0]).status.tolist() == [0, 0]
+    ids, ones = torch.tensor([3, 4], device="cuda"), torch.ones(2, dtype=torch.int32, device="cuda")
+    for t, lengths, status in ((0, [512, 1], [0, 0]), (1, [512, 2], [2, 0])):
+        logits = m.decode_paged(ids, cache, ones)
+        assert cache.lengths.tolist() == lengths and cache.status.tolist() == status and logits[1].isfinite().all()
+    check_status()
+
+
+def test_a_cache_holds_as_many_tokens_as_it_was_made_for():
+    m = _model(1)
+    cache = m.new_paged_cache(1, n_pages=10, page_size=16, max_tokens=20)
+    assert cache.capacity == 20
+    one = torch.ones(1, dtype=torch.int32, device="cuda")
+    for t in range(22):
+        m.decode_paged(torch.tensor([7], device="cuda"), cache, one)
+        assert (cache.lengths.item(), cache.status.item()) == (min(t + 1, 20), 0 if t < 20 else 2)
+    for page_size, max_tokens in ((16, -1), (0, 20)):
+        with pytest.raises(ValueError):
+            m.new_paged_cache(1, 10, page_size, max_tokens)
+
+
 def test_a_step_of_a_batch_together():
     """Plan, decode, settings, sampling: the step of a server, for requests that each have settings of their own, against the plain formulas on the same logits."""
     import paged_cases as ref

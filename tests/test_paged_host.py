@@ -43,6 +43,12 @@ def test_page_plan_refuses_a_status_over_its_inputs(built_lib):
             ops.plan_pages(i32(3), i32(3), i32(3, 4), i32(9), i32(1), 16, 3, status_out=wrong)
 
 
+def test_page_plan_refuses_a_negative_limit(built_lib):
+    import plz_native as P
+    base = {n: PTR + 0x1000 * i for i, (n, t) in enumerate(P.PagePlan._fields_) if t is C.c_void_p}
+    assert _call(P.lib().plz_page_plan, P.PagePlan, {**base, "ldt": 8, "B": 4, "width": 8, "page_size": 16, "n_pages": 100, "max_rows": 4, "row_pitch": 0})(max_tokens=-1) == SHAPE
+
+
 def test_page_write_refusals(built_lib):
     import plz_native as P
     base = dict(k=PTR, v=PTR, ldk=64, ldv=64, k_pages=PTR, v_pages=PTR, page_stride=1024, tok_stride=64, slots=PTR, rows=3, row_bytes=64, page_size=16, n_pages=5)
