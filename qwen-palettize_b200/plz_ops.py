@@ -768,6 +768,7 @@ def decode_hidden(ids: torch.Tensor, embed: torch.Tensor, layers, names, norms, 
 def embed_gather(table: torch.Tensor, ids: torch.Tensor) -> torch.Tensor:
     """table[ids] for a bf16 [vocab, width] table and int64 ids (any shape); returns bf16 [ids.numel(), width]."""
     assert table.dtype == torch.bfloat16 and table.dim() == 2 and table.stride(1) == 1 and ids.dtype == torch.int64
+    P._need_cuda(table, ids)
     flat = ids.reshape(-1).contiguous()
     out = torch.empty(flat.numel(), table.shape[1], dtype=torch.bfloat16, device=table.device)
     P.check(P.lib().plz_embed_gather(table.data_ptr(), table.stride(0), flat.data_ptr(), flat.numel(), table.shape[1], table.shape[0],

@@ -136,6 +136,13 @@ def test_binding_refusals(built_lib):
                 f(**{**good, **kw})
 
 
+def test_tokens_in_host_memory_are_refused_ahead_of_the_library(built_lib):
+    import plz_native as P
+    import plz_ops as ops
+    with pytest.raises(P.PlzError, match="CUDA tensors only"):
+        ops.embed_gather(torch.zeros(4, 64, dtype=torch.bfloat16), torch.zeros(2, dtype=torch.int64))
+
+
 def test_the_plain_plan():
     """By hand: two requests that share five free pages with one that ends, and a third that comes too late."""
     table, free = [[4, -1, -1], [7, 8, -1], [-1, -1, -1], [9, -1, -1]], [0, 1, 2, 3, 5, -1, -1, -1, -1, -1]
