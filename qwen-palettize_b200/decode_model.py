@@ -84,12 +84,21 @@ class PagedKVCache:
         return ops.plan_pages(self.lengths, new_tokens, self.table, self.free_pages, self.n_free, self.page_size, max_rows, row_pitch, lengths_out=self.lengths, n_free_out=self.n_free,
                               status_out=self.status, max_tokens=self.max_tokens)
 
+    def check(self, n_layers: int, width: int, device, what: str):
+        """A ValueError for what has other layers or columns than the pages: ahead of a plan, which lengthens the requests."""
+        mine = (self.k.shape[0], self.k.shape[3], self.k.device)
+        if (n_layers, width, device) != mine:
+            raise ValueError(f"{what} of {n_layers} layers of {width} columns on {device}, pages of {mine[0]} layers of {mine[1]} on {mine[2]}")
+
     def fill(self, cache: KVCache, requests) -> ops.PagePlan:
         """The filled positions of `cache`, one sequence for each of `requests` (row numbers in increasing order) that hold nothing yet: prompts' keys and values after prefill. The plan's
         status says who got no pages."""
         requests = list(requests)
         if cache.k.shape[1] != len(requests) or sorted(set(requests)) != requests or not all(0 <= r < self.requests for r in requests):
             raise ValueError(f"{cache.k.shape[1]} sequences for the requests {requests} of {self.requests}")
+        self.check(cache.k.shape[0], cache.k.shape[3], cache.k.device, "a cache")
+        if cache.k.dtype != self.k.dtype or cache.v.dtype != self.v.dtype or cache.v.shape != cache.k.shape or cache.v.device != cache.k.device:
+            raise ValueError(f"keys {cache.k.dtype} {tuple(cache.k.shape)} and values {cache.v.dtype} {tuple(cache.v.shape)} for pages of {self.k.dtype}")
         n = cache.length
         new = torch.zeros(self.requests, dtype=torch.int32)
         new[requests] = n
@@ -281,6 +290,9 @@ class PalettizedQwen:
             raise ValueError(f"requests of {cache.capacity} tokens, but positions up to {self.cos.shape[0]}")
         if ids.numel() != B or new_tokens.numel() != B:
             raise ValueError(f"{ids.numel()} tokens and {new_tokens.numel()} counts for {B} requests")
+        if ids.dtype != torch.int64 or ids.device != self.embed.device:
+            raise ValueError(f"tokens: int64 on {self.embed.device}, not {ids.dtype} on {ids.device}")
+        cache.check(c.n_layers, c.n_kv_heads * c.head_dim, self.embed.device, "a model")
         p = cache.plan(new_tokens, B, row_pitch=1)
         at = p.positions.clamp(min=0).long()
         cos, sin = self.cos[at], self.sin[at]

@@ -162,6 +162,26 @@ def test_a_cache_holds_as_many_tokens_as_it_was_made_for():
             m.new_paged_cache(1, 10, page_size, max_tokens)
 
 
+def test_what_is_refused_leaves_the_cache_as_it_was():
+    """Tokens of another type or on the host, a cache or prompts of another model: no request grows by tokens whose keys were never written, no page is lost."""
+    import decode_model as D
+    m = _model(1)
+    cache = m.new_paged_cache(2, 10, 16, 64)
+    ones = torch.ones(2, dtype=torch.int32, device="cuda")
+    ids = torch.tensor([3, 4], device="cuda")
+    m.decode_paged(ids, cache, ones)
+    deep, wide = _model(1, n_layers=3), _model(1, n_kv_heads=4)
+    kv = lambda m: D.KVCache(*(m.new_cache(2, 64).k for _ in range(2)), length=16)
+    calls = [lambda: m.decode_paged(ids.int(), cache, ones), lambda: m.decode_paged(ids.cpu(), cache, ones), lambda: deep.decode_paged(ids, cache, ones), lambda: wide.decode_paged(ids, cache, ones),
+             lambda: cache.fill(kv(deep), [0, 1]), lambda: cache.fill(kv(wide), [0, 1]), lambda: cache.fill(D.KVCache(*(t.float() for t in (kv(m).k, kv(m).v)), length=16), [0, 1])]
+    for i, call in enumerate(calls):
+        with pytest.raises(ValueError):
+            call()
+        assert cache.lengths.tolist() == [1, 1] and cache.n_free.item() == 8, i
+    m.decode_paged(ids, cache, ones)
+    assert cache.lengths.tolist() == [2, 2]
+
+
 def test_a_step_of_a_batch_together():
     """Plan, decode, settings, sampling: the step of a server, for requests that each have settings of their own, against the plain formulas on the same logits."""
     import paged_cases as ref
