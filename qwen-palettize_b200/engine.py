@@ -156,7 +156,7 @@ class Engine:
             kw.update(bias_ids=r.bias[0], bias=r.bias[1])
         ids = p.allowed(list(r.out)) if p.allowed is not None else None
         if ids is not None:
-            ids = torch.tensor(sorted(set(ids)), dtype=torch.int64)
+            ids = torch.tensor(sorted({int(t) for t in (ids.tolist() if hasattr(ids, "tolist") else ids)}), dtype=torch.int64)      # numbers: equal elements of a tensor are different objects
             if ids.numel() == 0 or ids[0] < 0 or ids[-1] >= V:
                 raise ValueError(f"request {r.rid!r}: no token is allowed, or one outside the vocabulary of {V}")
             words = torch.zeros((V + 31) // 32, dtype=torch.int64)

@@ -274,6 +274,15 @@ def test_a_request_that_fails_ends_alone():
     assert eng.run()[good] == want and bad not in eng.finished and bad not in eng.pool
 
 
+@pytest.mark.parametrize("words", [lambda: torch.tensor([7, 7]), lambda: torch.tensor([7, 7], device="cuda"), lambda: [7, 7],
+                                   lambda: __import__("numpy").array([7, 7])], ids=["tensor", "device", "list", "array"])
+def test_allowed_tokens_of_any_kind(words):
+    """The same token several times is allowed once, whatever holds the numbers."""
+    from engine import Engine, SamplingParams
+    out = Engine(_model(3), 64).generate([[5, 17]], SamplingParams(max_new=6, allowed=lambda out: words()))[0]
+    assert out == [7] * 6
+
+
 def test_settings_from_the_command_line(tmp_path, capsys):
     import cli
     import model_registry as R
