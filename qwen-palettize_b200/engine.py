@@ -51,6 +51,7 @@ class Engine:
         self.model, self.portion, self.max_live = model, portion, max_live
         self.pool = StatePool(model, max_tokens)
         self.waiting, self.live, self.finished = deque(), deque(), {}
+        self.failed = {}             # request id: (exception, tokens generated so far) of requests that ended so
         self._next = 0
 
     # ---- the step ----------------------------------------------------------------------------------------------------
@@ -116,9 +117,11 @@ class Engine:
         if logits is not None and r.params.max_new > 0:
             try:
                 self._take(r, logits)
-            except Exception:            # its settings failed: it ends, the others go on with the next call
+            except Exception as e:       # its settings failed: it ends, the others go on with the next call
                 self.live.remove(r)
                 self.end(r.rid)
+                self.failed[r.rid] = (e, r.out)
+                e.add_note(f"request {r.rid!r} after {len(r.out)} tokens")
                 raise
         if r.done or (r.fed == len(r.prompt) and len(r.out) >= r.params.max_new):
             self.live.remove(r)
@@ -164,14 +167,35 @@ class Engine:
             kw["mask"] = torch.where(words >= 1 << 31, words - (1 << 32), words).to(torch.int32).view(1, -1).to(dev)
         return S.adjust_logits(logits, **kw)
 
+    def cancel(self, rid):
+        """Whatever has become of a submitted request, nothing of it stays."""
+        self.waiting = deque(r for r in self.waiting if r.rid != rid)
+        self.live = deque(r for r in self.live if r.rid != rid)
+        self.end(rid)
+        self.finished.pop(rid, None)
+        self.failed.pop(rid, None)
+
     def run(self) -> dict:
-        """Until every submitted request is finished: {request id: generated tokens} of all finished so far."""
+        """Until every submitted request is finished: {request id: generated tokens} of all finished so far. A request that fails raises and is in `failed`; the next call goes on with the others."""
         while self.run_one():
             pass
         return self.finished
 
     def generate(self, prompts, params: SamplingParams | None = None):
-        """Generated tokens of every prompt, in order."""
-        ids = [self.submit(p, params) for p in prompts]
-        done = self.run()
-        return [done.pop(i) for i in ids]
+        """Generated tokens of every prompt, in order. Where one of them fails, none of them stays."""
+        ids = []
+        try:
+            for p in prompts:
+                ids.append(self.submit(p, params))
+            while True:
+                try:
+                    if not self.run_one():
+                        return [self.finished.pop(i) for i in ids]
+                except Exception as e:
+                    rid = next((i for i, (error, _) in self.failed.items() if error is e), None)
+                    if rid is None or rid in ids:
+                        raise            # else the request of another caller, who finds it in `failed`
+        except BaseException:
+            for i in ids:
+                self.cancel(i)
+            raise

@@ -283,6 +283,45 @@ def test_allowed_tokens_of_any_kind(words):
     assert out == [7] * 6
 
 
+def test_a_generation_that_fails_leaves_nothing_behind():
+    """One of three prompts fails: none of them runs on in the next generation, none keeps a state or a result; the error names the request. Requests of others are untouched."""
+    from engine import Engine, SamplingParams
+    m = _model(3)
+    want = Engine(m, 64).generate([[9, 4, 2], [8]], SamplingParams(max_new=4))
+    eng = Engine(m, 64, max_live=2)
+    other = eng.submit([9, 4, 2], SamplingParams(max_new=4))
+
+    def fails(out):
+        if len(out) == 2:
+            raise KeyError("no rule")
+    with pytest.raises(KeyError, match="no rule") as e:
+        eng.generate([[5, 17], [6], [7, 7]], SamplingParams(max_new=6, allowed=fails))
+    assert "2 tokens" in e.value.__notes__[0] and not eng.failed
+    assert eng.generate([[8]], SamplingParams(max_new=4)) == want[1:]
+    assert eng.finished == {other: want[0]} and not eng.live and not eng.waiting and not eng.pool.live
+    with pytest.raises(ValueError):                # the second prompt is refused: the first one does not stay
+        eng.generate([[5], []], SamplingParams(max_new=4))
+    assert not eng.live and not eng.waiting and not eng.pool.live
+
+
+def test_a_request_that_fails_is_recorded_and_stops_nobody_else():
+    from engine import Engine, SamplingParams
+    m = _model(3)
+    want = Engine(m, 64).generate([[9, 4, 2], [8]], SamplingParams(max_new=4))
+    eng = Engine(m, 64)
+    bad = eng.submit([5, 17], SamplingParams(max_new=6, allowed=lambda out: range(1000) if len(out) < 2 else []))
+    assert eng.generate([[9, 4, 2], [8]], SamplingParams(max_new=4)) == want       # whose request it is not
+    error, tokens = eng.failed.pop(bad)
+    assert isinstance(error, ValueError) and repr(bad) in error.__notes__[0] and len(tokens) == 2
+    eng.submit([5, 17], SamplingParams(max_new=6, allowed=lambda out: []))
+    assert eng.generate([], None) == [] and len(eng.failed) == 1
+    gone = [eng.submit([5], SamplingParams(max_new=3)) for _ in range(2)]
+    eng.run_one()
+    for rid in gone + gone:
+        eng.cancel(rid)
+    assert not eng.live and not eng.waiting and not eng.pool.live and not eng.run()
+
+
 def test_settings_from_the_command_line(tmp_path, capsys):
     import cli
     import model_registry as R
