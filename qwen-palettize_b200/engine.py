@@ -5,7 +5,9 @@ first-come scheduler that cuts prompts into portions and interleaves decoding, a
 """
 from __future__ import annotations
 
+import math
 from collections import deque
+from ctypes import c_float
 from dataclasses import dataclass, field
 
 import torch
@@ -80,8 +82,14 @@ class Engine:
         params = params or SamplingParams()
         if not prompt:
             raise ValueError("empty prompt")
-        if not params.repetition > 0.0:
+        r, p, f = (c_float(v).value for v in (params.repetition, params.presence, params.frequency))      # as the kernel takes them
+        if not 0.0 < r < math.inf:
             raise ValueError("the repetition penalty is a positive factor")
+        total = {}
+        for t, v in params.bias:
+            total[t] = total.get(t, 0.0) + c_float(v).value
+        if any(math.isnan(v - p - f) for v in (0.0, *total.values())):
+            raise ValueError("presence, frequency and biases that add up to no number")
         if any(not 0 <= t < self.model.vocab for t, _ in params.bias):
             raise ValueError(f"a bias for a token outside the vocabulary of {self.model.vocab}")
         if len(params.bias) > 4096:

@@ -143,6 +143,20 @@ def test_tokens_in_host_memory_are_refused_ahead_of_the_library(built_lib):
         ops.embed_gather(torch.zeros(4, 64, dtype=torch.bfloat16), torch.zeros(2, dtype=torch.int64))
 
 
+def test_settings_that_make_no_number_are_refused_with_the_request(built_lib):
+    from types import SimpleNamespace
+    from engine import Engine, SamplingParams
+    eng = Engine(SimpleNamespace(vocab=100), 64)
+    nan, inf = float("nan"), float("inf")
+    for kw in ({"repetition": nan}, {"repetition": inf}, {"repetition": 1e39}, {"repetition": 1e-46}, {"repetition": -1.0}, {"presence": nan}, {"frequency": nan}, {"presence": inf, "frequency": -inf},
+               {"presence": 1e39, "frequency": -1e39}, {"bias": ((3, nan),)}, {"bias": ((3, inf), (3, -inf))}, {"bias": ((3, inf),), "presence": inf}):
+        with pytest.raises(ValueError):
+            eng.submit([1], SamplingParams(**kw))
+    assert not eng.waiting
+    for kw in ({"repetition": 1e38}, {"repetition": 1e-45}, {"presence": inf}, {"frequency": -3.0}, {"bias": ((3, -inf), (4, inf), (3, 1.0))}, {"bias": ((3, -inf),), "presence": inf}):
+        eng.submit([1], SamplingParams(**kw))
+
+
 def test_the_plain_plan():
     """By hand: two requests that share five free pages with one that ends, and a third that comes too late."""
     table, free = [[4, -1, -1], [7, 8, -1], [-1, -1, -1], [9, -1, -1]], [0, 1, 2, 3, 5, -1, -1, -1, -1, -1]
