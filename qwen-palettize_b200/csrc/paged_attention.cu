@@ -60,9 +60,11 @@ __device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uin
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
+constexpr int kMostTokens = 0x7FFFFFC0;     // of a request: steps are counted by rounding up, and a step's last token is computed before it is compared, both within 31 of the length
+
 // tokens of a request that are attended to
 __device__ __forceinline__ int tokens_of(const PagedParams& p, int len) {
-    const long long room = (long long)p.width * p.page;
+    const long long room = min((long long)p.width * p.page, (long long)kMostTokens);
     return len < 0 ? 0 : (long long)len > room ? (int)room : len;
 }
 
@@ -508,7 +510,7 @@ paged_attn_kernel(const PagedParams p) {
     // ---- requests without tokens, and lengths that there cannot be
     for (int b = empty || p.bad ? cta : p.B; b < p.B; b += ctas) {
         const int len = p.lengths[b];
-        if (tid == 0 && p.bad && (len < 0 || len > (long long)p.width * p.page)) *p.bad = 1;
+        if (tid == 0 && p.bad && len != tokens_of(p, len)) *p.bad = 1;
         if (!empty || tokens_of(p, len) > 0) continue;
         for (int x = tid * 8; x < p.Hq * D; x += NW * 256) *reinterpret_cast<uint4*>(p.out + (long long)b * p.ldo + x) = make_uint4(0u, 0u, 0u, 0u);
     }

@@ -399,6 +399,22 @@ def test_no_requests():
     assert (ops.attention_decode_paged(q, kp[:0], vp[:0], table[:, :0], L, 8, 2) == 0).all()
 
 
+def test_lengths_next_to_the_largest_number():
+    """A table with room for 2^31 tokens, all of them one page: lengths up to 2^31 - 64 are served, longer ones cut to that. Equal weights over the page's values, sums of them whole."""
+    import plz_ops as ops
+    page, most = 1 << 16, 2 ** 31 - 64
+    kp = torch.zeros(1, page, 64, dtype=torch.bfloat16, device="cuda")
+    vp = torch.ones_like(kp)
+    vp[:, :, 1] = -2.0
+    table = torch.zeros(1, 1 << 15, dtype=I32, device="cuda")
+    q = torch.ones(1, 128, dtype=torch.bfloat16, device="cuda")
+    bad = torch.zeros(1, dtype=I32, device="cuda")
+    for n, cut in ((most - 1, 0), (most, 0), (most + 1, 1), (2 ** 31 - 1, 1)):
+        got = ops.attention_decode_paged(q, kp, vp, table, _dev([n]), 2, 1, 64, bad=bad).view(2, 64)
+        assert bad.item() == cut and (got[:, 0] == 1).all() and (got[:, 1] == -2).all() and (got[:, 2:] == 1).all(), n
+        bad.zero_()
+
+
 def test_pool_past_four_gigabytes():
     """Offsets that no 32-bit count of elements or bytes holds: the request's pages lie at both ends of a pool of 6 GB per tensor."""
     import plz_ops as ops
