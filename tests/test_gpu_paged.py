@@ -240,6 +240,51 @@ def test_attention_with_many_steps(hq, hk, d, page, B, T):
     assert all(torch.equal(got[0], x) for x in got[1:])
 
 
+@pytest.mark.parametrize("hq,hk,d,page,lengths", [(4, 1, 128, 16, [400003]), (8, 2, 64, 24, [250001, 17, 130000]), (4, 1, 256, 64, [120007]), (12, 1, 128, 16, [90001, 300007])])
+def test_long_requests_have_every_step_in_them(hq, hk, d, page, lengths):
+    """Column c of a value is 1 in the c-th of d equal stretches of its request and 0 elsewhere, so result c is the weight of that stretch, about 1 / d: one step (16 tokens, 32 of 64-wide heads) more or
+    less changes it by 16 d / T of itself (32 d / T), 5e-3 or more here. Its rounding to bf16 is half of finfo.eps = 2^-7 of itself at most, 2^-8 = 3.9e-3. Head 0 weighs all tokens alike, the others by random scores. Other errors, by T tokens cut in stretches of
+    n = T Hkv / 16 / SMs / 4 + 1 steps or fewer: a weight 2 (d + 4) 2^-23 sum |q k| + 2^-21, a sum of weights or products 2^-23 for each of a lane's 16 n terms and of 400 parts."""
+    import plz_ops as ops
+    g = torch.Generator(device="cuda").manual_seed(d + page)
+    B, width = len(lengths), -(-max(lengths) // page)
+    table = torch.randperm(B * width, generator=g, device="cuda").to(I32).view(B, width)
+    kp, vp = (torch.full((B * width, page, hk * d), float("nan"), dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    q = (torch.randn(B, hk, hq // hk, d, generator=g, device="cuda") / 2).bfloat16()
+    q[:, :, 0] = 0
+    sms = torch.cuda.get_device_properties(0).multi_processor_count
+    steps = sum(lengths) * hk // 16 // sms // 4 + 1
+    cases = []
+    for b, n in enumerate(lengths):
+        pos = torch.arange(n, device="cuda")
+        at = table[b, pos // page].long() * page + pos % page
+        k = torch.randn(n, hk * d, generator=g, device="cuda").bfloat16()
+        part = (pos * d // n)
+        kp.view(-1, hk * d)[at] = k
+        vp.view(-1, hk * d)[at] = torch.nn.functional.one_hot(part, d).repeat(1, hk).bfloat16()
+        cases.append((n, part, k.view(n, hk, d)))
+    got = ops.attention_decode_paged(q.view(B, -1), kp, vp, table, _dev(lengths), hq, hk, d).double().view(B, hk, hq // hk, d)
+    check_status()
+
+    def weights(w, part):                       # per head the share of every stretch
+        return torch.zeros(hk, hq // hk, d, dtype=torch.float64, device="cuda").index_add_(2, part, w / w.sum(-1, keepdim=True))
+    for b, (n, part, k) in enumerate(cases):
+        s = torch.einsum("hgd,nhd->hgn", q[b].double(), k.double()) * d ** -0.5
+        w = (s - s.amax(-1, keepdim=True)).exp()
+        want = weights(w, part)
+        size = torch.einsum("hgd,nhd->hgn", q[b].double().abs(), k.double().abs()).amax(-1, keepdim=True) * d ** -0.5
+        rel = 2.0 ** -8 * (1 + 2.0 ** -8) + 2 * (2 * (d + 4) * 2.0 ** -23 * size + 2.0 ** -21 + (16 * min(steps, -(-n // 16)) + 400) * 2.0 ** -23)
+        right = lambda x: bool(((x - want).abs() <= rel * want).all())
+        assert right(got[b]), (b, float(((got[b] - want).abs() / (rel * want)).nan_to_num().max()))
+        # what the bound has to notice: nothing, half of the request, and where all tokens weigh alike one step left out
+        if n > 1000:
+            half, step = w.clone(), w.clone()
+            half[..., n // 2:] = 0
+            tok = 32 if d == 64 else 16
+            step[..., n // 3 // tok * tok:][..., :tok] = 0
+            assert not any(right(x) for x in (torch.zeros_like(want), weights(half, part), weights(step, part)))
+
+
 @pytest.mark.parametrize("B", [2, 31, 32, 33, 64])
 @pytest.mark.parametrize("hq,hk,d", [(8, 2, 128), (20, 1, 64), (4, 4, 256)])
 @pytest.mark.parametrize("holes", ["none", "ends", "inside", "most"])
