@@ -623,7 +623,8 @@ int32_t plz_sample(const float* logits, int64_t ld, int32_t rows, int32_t V, flo
  * plz_attn_decode_paged: attention of one new token per request (its key and value stored already): out[b, h] = softmax(q[b, h] . K[0 .. lengths[b]) * scale) V[0 .. lengths[b])
  *   over the request's pages, key / value head h / (Hq / Hkv). bf16, q and out [B, Hq * head_dim], pools [n_pages, page_size, Hkv * head_dim] with the element strides
  *   between pages and between rows, head_dim 64, 128 or 256. lengths[b] <= 0 gives zeros. Nothing behind a request's length is read into the result. A page outside the pool
- *   is left out of the softmax and a length past `width` pages or 2^31 - 64 is cut, either of them (and a negative length) stores 1 to *bad (device int32, may be NULL); values are finite.
+ *   is left out of the softmax and a length past `width` pages or 2^31 - 64 is cut, either of them (and a negative length) stores 1 to *bad (device int32, may be NULL); a request of
+ *   length > 0 none of whose pages lies in the pool has no weight to divide by: its row is NaN, not zeros. Values are finite.
  *   ws: plz_attn_decode_paged_ws_bytes, 16-byte aligned, for any B and lengths; calls that may run at the same time need one each. Bits repeat from run to run; a request's may change with the other requests'
  *   lengths, which move the places where its sums are cut.
  * plz_adjust_logits: out = logits [rows, V] (dtype 0 bf16, 1 fp32, computed in fp32, out may be logits with the same pitch) after, in this order,

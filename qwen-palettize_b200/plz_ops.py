@@ -699,7 +699,7 @@ def attention_decode_paged(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torc
                            head_dim: int = 128, scale: float | None = None, out: torch.Tensor | None = None, bad: torch.Tensor | None = None) -> torch.Tensor:
     """Attention of one new token per request over the request's own length of cached tokens (its own among them). q bf16 [B, n_heads * head_dim], pools bf16
     [n_pages, page_size, n_kv_heads * head_dim], table int32 [B, width], lengths int32 [B] on the device (0: zeros). Returns bf16 [B, n_heads * head_dim]. bad (int32 [1]) is set to 1
-    where a page lies outside the pool (its tokens are left out) or a length outside the table."""
+    where a page lies outside the pool (its tokens are left out; all of a request's: its row is NaN) or a length outside the table."""
     got = P.calls().attention_decode_paged(q, k_pages, v_pages, table, lengths, n_heads, n_kv_heads, head_dim, scale, out, bad)
     if got is not None:
         return got

@@ -444,6 +444,23 @@ def test_no_requests():
     assert (ops.attention_decode_paged(q, kp[:0], vp[:0], table[:, :0], L, 8, 2) == 0).all()
 
 
+@pytest.mark.parametrize("lengths", [[16] * 700, [9000, 5, 9000], [2049], [40] * 33], ids=["by a warp", "across CTAs", "one request", "small batch"])
+@pytest.mark.parametrize("page", [0, 2 ** 31 - 1, -1])
+def test_requests_without_any_page_in_the_pool(page, lengths):
+    """No weight at all: NaN in their rows wherever they are finished, the others as they are."""
+    import plz_ops as ops
+    q, kp, vp, table, L = _case(len(lengths), lengths, 8, 2, 128, 16)
+    want, err = ref.attention(q, kp, vp, table, L, 8, 2, 128)
+    gone = torch.arange(len(lengths)) % 2 == 0
+    table[gone.cuda()] = page if page else kp.shape[0]
+    bad = torch.zeros(1, dtype=I32, device="cuda")
+    got = ops.attention_decode_paged(q, kp, vp, table, L, 8, 2, bad=bad)
+    check_status()
+    assert got[gone.cuda()].isnan().all() and bad.item() == 1
+    if not gone.all():
+        _close(got.cpu()[~gone], want.cpu()[~gone], err.cpu()[~gone])
+
+
 def test_lengths_next_to_the_largest_number():
     """A table with room for 2^31 tokens, all of them one page: lengths up to 2^31 - 64 are served, longer ones cut to that. Equal weights over the page's values, sums of them whole."""
     import plz_ops as ops
