@@ -10,6 +10,8 @@
 //     a group here, and would need the warps to meet in every step; the tensor pipe is 19 % busy at the speed of memory as it is.
 //     Weights are three bf16 terms of the fp32 value, all 24 bits of it (two terms, 16 bits, differed from the sums in fp32 in the last bit of 0.2 % of the results). With up to 8 query heads
 //     the second terms are rows 8 to 15 of the same product and cost nothing, the third are a product of their own: 256 short requests 39.9 -> 41.0 us, long ones within 1 %.
+//     A step's sums are added to the others in fp32, rounded to nearest: the tensor cores' own accumulators cut every sum, and after n steps n 2^-24 of it is gone (32 requests of 131072 tokens, 3500
+//     steps a warp: 2.1 % of the results off in their last bit, 0.006 % this way). It costs 1 %, 7 % with heads of 256, where registers spill (33.8 -> 36.3 us for 32 requests of up to 4096 tokens).
 //     The reference of the exponentials moves when a row's maximum has grown by more than 2^8.
 //     A head that a warp finishes alone goes to `out`; parts meet in shared memory at the end, parts that cross CTAs go to the workspace, two per CTA at most.
 //   paged_join_kernel  one block per CTA of the first kernel and query head of a group joins the parts of the head that began there and went on; most have nothing to do.
@@ -62,6 +64,12 @@ __device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uin
 
 constexpr int kMostTokens = 0x7FFFFFC0;     // of a request: steps are counted by rounding up, and a step's last token is computed before it is compared, both within 31 of the length
 
+// the same without sums to add to
+__device__ __forceinline__ void mma0(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+                 : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+}
+
 // tokens of a request that are attended to
 __device__ __forceinline__ int tokens_of(const PagedParams& p, int len) {
     const long long room = min((long long)p.width * p.page, (long long)kMostTokens);
@@ -110,6 +118,8 @@ struct Cfg {
     static constexpr int kSmem = NW * kWarp;
     static_assert(kPart * 4 <= kRing, "the last part lies in the ring");
 };
+struct Yes { static constexpr bool value = true; };
+struct No { static constexpr bool value = false; };
 struct PartMeta { int b, item, flags, rest; };      // flags 1: valid, 2: holds the head's first step, 4: holds its last; rest: steps behind it
 
 template <typename C>
@@ -372,22 +382,30 @@ paged_attn_kernel(const PagedParams p) {
                 for (int n = 0; n < NT; n += 2)
 #pragma unroll
                     for (int j = 0; j < D / 16; j += 2) {
-                        // four independent products between two that add to the same sums
+                        // four independent products between two that add to the same sums, which are those of this step
                         uint32_t b[2][4];
 #pragma unroll
                         for (int i = 0; i < 2; ++i) ldm4t(b[i], base + n * 8 * (D * 2) + (((2 * (j + i) + upper) ^ (lane & 7)) << 4));
-                        auto add = [&](uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3) {
+                        float sum[4][4];
+                        auto add = [&](auto first, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3) {
 #pragma unroll
-                            for (int i = 0; i < 4; ++i) mma(acc[2 * j + i], a0, a1, a2, a3, b[i >> 1][2 * (i & 1)], b[i >> 1][2 * (i & 1) + 1]);
+                            for (int i = 0; i < 4; ++i) {
+                                if constexpr (first.value) mma0(sum[i], a0, a1, a2, a3, b[i >> 1][2 * (i & 1)], b[i >> 1][2 * (i & 1) + 1]);
+                                else mma(sum[i], a0, a1, a2, a3, b[i >> 1][2 * (i & 1)], b[i >> 1][2 * (i & 1) + 1]);
+                            }
                         };
                         if constexpr (NR == 1) {
-                            add(hi[n][0], mid[n][0], hi[n + 1][0], mid[n + 1][0]);
-                            add(lo[n][0], 0u, lo[n + 1][0], 0u);
+                            add(Yes{}, hi[n][0], mid[n][0], hi[n + 1][0], mid[n + 1][0]);
+                            add(No{}, lo[n][0], 0u, lo[n + 1][0], 0u);
                         } else {
-                            add(hi[n][0], hi[n][1], hi[n + 1][0], hi[n + 1][1]);
-                            add(mid[n][0], mid[n][1], mid[n + 1][0], mid[n + 1][1]);
-                            add(lo[n][0], lo[n][1], lo[n + 1][0], lo[n + 1][1]);
+                            add(Yes{}, hi[n][0], hi[n][1], hi[n + 1][0], hi[n + 1][1]);
+                            add(No{}, mid[n][0], mid[n][1], mid[n + 1][0], mid[n + 1][1]);
+                            add(No{}, lo[n][0], lo[n][1], lo[n + 1][0], lo[n + 1][1]);
                         }
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) acc[2 * j + i][e] += sum[i][e];
                     }
             }
             const bool over = step + 1 == seen, done = (st.z + 1) * TOK >= st.w;

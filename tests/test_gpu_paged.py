@@ -285,6 +285,30 @@ def test_long_requests_have_every_step_in_them(hq, hk, d, page, lengths):
             assert not any(right(x) for x in (torch.zeros_like(want), weights(half, part), weights(step, part)))
 
 
+@pytest.mark.parametrize("hq,hk,d", [(8, 1, 128), (12, 1, 128), (8, 1, 64), (8, 1, 256), (12, 1, 64), (12, 1, 256)])
+def test_long_sums_do_not_drift(hq, hk, d):
+    """Ten thousand steps a warp, over pages that come again and again: sums that are rounded to nearest are off by about sqrt(n) 2^-25 of themselves after n steps, 6 times that or less, and weights by
+    2^-21 (exponential and exponent); an error e moves a value over a border between two bf16 numbers, 2^-8 apart or more, in 2 e 2^8 of all cases or fewer. Sums that are cut instead lose n 2^-24."""
+    import plz_ops as ops
+    tok, warps = (32 if d == 64 else 16), (4 if d == 256 else 8) * torch.cuda.get_device_properties(0).multi_processor_count
+    B, n_pages, page, n = 8, 256, 64, 10000
+    width = n * warps * tok // page // B // hk
+    g = torch.Generator(device="cuda").manual_seed(d)
+    table = torch.randint(0, n_pages, (B, width), generator=g, device="cuda").int()
+    kp = torch.randn(n_pages, page, hk * d, generator=g, device="cuda").bfloat16()
+    vp = (1 + torch.rand(n_pages, page, hk * d, generator=g, device="cuda")).bfloat16()
+    q = torch.randn(B, hq * d, generator=g, device="cuda").bfloat16()
+    got = ops.attention_decode_paged(q, kp, vp, table, torch.full((B,), width * page, dtype=I32, device="cuda"), hq, hk, d).view(B, hk, hq // hk, d)
+    check_status()
+    often = torch.stack([torch.bincount(table[b], minlength=n_pages) for b in range(B)]).repeat_interleave(page, 1).double()
+    k, v = (t.view(-1, hk, d).double().transpose(0, 1) for t in (kp, vp))
+    s = q.view(B, hk, hq // hk, d).double() @ k.transpose(1, 2) * d ** -0.5
+    w = (s - s.amax(-1, keepdim=True)).exp() * often[:, None, None]
+    want = (w / w.sum(-1, keepdim=True)) @ v
+    e = 6 * n ** 0.5 * 2.0 ** -25 + 2.0 ** -21
+    assert float((got.double() != want.bfloat16().double()).double().mean()) <= 2 * e * 2 ** 8
+
+
 @pytest.mark.parametrize("B", [2, 31, 32, 33, 64])
 @pytest.mark.parametrize("hq,hk,d", [(8, 2, 128), (20, 1, 64), (4, 4, 256)])
 @pytest.mark.parametrize("holes", ["none", "ends", "inside", "most"])
