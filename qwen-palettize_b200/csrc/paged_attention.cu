@@ -7,25 +7,28 @@
 //     tokens are asked for four steps ahead, its keys and values two steps ahead, all by cp.async through a ring of the warp's own, which goes on over the ends of heads and requests: nothing waits
 //     between short requests, and there is no barrier until a CTA's warps meet at the end.
 //     Scores and sums are mma.sync m16n8k16 on fragments read by ldmatrix: the query heads are the 16 rows, the tokens the columns. tcgen05 has 64 rows at least, for the 4 query heads of
-//     a group here, and would need the warps to meet in every step; the tensor pipe is 19 % busy at the speed of memory as it is.
+//     a group here, and would need the warps to meet in every step; the tensor pipe is 28 % busy at the speed of memory as it is.
 //     Weights are three bf16 terms of the fp32 value, all 24 bits of it (two terms, 16 bits, differed from the sums in fp32 in the last bit of 0.2 % of the results). With up to 8 query heads
 //     the second terms are rows 8 to 15 of the same product and cost nothing, the third are a product of their own: 256 short requests 39.9 -> 41.0 us, long ones within 1 %.
-//     A step's sums are added to the others in fp32, rounded to nearest: the tensor cores' own accumulators cut every sum, and after n steps n 2^-24 of it is gone (32 requests of 131072 tokens, 3500
-//     steps a warp: 2.1 % of the results off in their last bit, 0.006 % this way). It costs 1 %, 7 % with heads of 256, where registers spill (33.8 -> 36.3 us for 32 requests of up to 4096 tokens).
+//     The accumulators of the products cut what falls below their last bit instead of rounding it: after n steps about n 2^-24 of a sum is gone (32 requests of 131072 tokens, 3500 steps a warp:
+//     2.1 % of the results off in their last bit). So a warp's sums of 64 steps are added to earlier ones in fp32, rounded to nearest, which a lane keeps for itself in the workspace (0.02 %;
+//     2 x 131072 tokens 165.6 -> 168.6 us; a step's sums added by themselves 166.5, but 182 where 172 is reached with the clocks of sustained load); with heads of 256, those of a step.
 //     The reference of the exponentials moves when a row's maximum has grown by more than 2^8.
 //     A head that a warp finishes alone goes to `out`; parts meet in shared memory at the end, parts that cross CTAs go to the workspace, two per CTA at most.
 //   paged_join_kernel  one block per CTA of the first kernel and query head of a group joins the parts of the head that began there and went on; most have nothing to do.
 //
-// Measured (query / key heads 32 / 8 of 128, pages of 16 or 64): 2 x 131072 tokens 160 us for 1.07 GB, 6.7 TB/s; 64 requests of up to 4096 tokens 96 us for 0.59 GB, 6.1 TB/s; 256 requests of up to
-// 300 tokens, 16 / 16 heads of 64, 37 us for 0.16 GB; one request of 2049 tokens 9 us, a chain of latencies: lengths, pages, keys, two meetings, a second launch.
-//   What is in flight matters: three steps a warp (196 KB of copies per SM) 187 and 110 us, since SMs then starve one another (their times spread over 73 to 95 us at equal work, which taking the
-//   work as it comes did not mend: its many parts cost as much as it gave); two steps (128 KB) 160 and 96; six warps of two steps 166 and 100.
+// Measured, replayed (query / key heads 32 / 8 of 128, pages of 16 or 64): 2 x 131072 tokens 166 to 169 us for 1.07 GB, 6.4 TB/s; 64 requests of up to 4096 tokens 99 us for 0.58 GB, 5.8 TB/s; 256 requests
+// of up to 300 tokens, 16 / 16 heads of 64, 39 us for 0.16 GB; one request of 2049 tokens 8.6 us, a chain of latencies: lengths, pages, keys, two meetings, a second launch. Heads 8 / 2 of 256,
+// 32 requests of up to 4096 tokens, 38 us for 0.12 GB; 32 / 2 of 128, 64 such requests, 44 us for 0.14 GB.
+//   What is in flight matters (before the third term and the kept sums): three steps a warp (196 KB of copies per SM) 187 and 110 us for the first two, since SMs then starve one another (their times
+//   spread over 73 to 95 us at equal work, which taking the work as it comes did not mend: its many parts cost as much as it gave); two steps (128 KB) 160 and 96; six warps of two steps 166 and 100.
 #include "plz_launch.h"
 
 namespace plz {
 namespace {
 
 constexpr int kSwitch = 2;               // steps that the change to another head counts on the line (0: 256 short requests 45 us; 1, 2: 37; 4: 39)
+constexpr int kCut = 64;                 // steps after which a warp's sums are kept elsewhere and begun anew
 constexpr float kGrow = 8.f;             // exponents (base 2) that a maximum may grow before the reference moves
 constexpr float kLog2e = 1.4426950408889634f;
 
@@ -37,7 +40,7 @@ struct PagedParams {
     const int* lengths;
     __nv_bfloat16* out; long long ldo;
     int* bad;
-    float* parts; int4* heads;           // workspace: parts, two of every CTA and one of each of its warps; {request, item in it, last CTA} of the head that goes on from every CTA
+    float4* kept; float* parts; int4* heads;      // workspace: sums that a warp keeps; parts, two of every CTA and one of each of its warps; {request, item in it, last CTA} of the head that goes on from every CTA
     int B, width, page, n_pages, Hq, Hkv, G, blocks, items;   // blocks of 16 query heads per key / value head, items = Hkv * blocks
     int shift;                           // log2(page), or -1
     float scale_log2e;
@@ -63,12 +66,6 @@ __device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uin
 }
 
 constexpr int kMostTokens = 0x7FFFFFC0;     // of a request: steps are counted by rounding up, and a step's last token is computed before it is compared, both within 31 of the length
-
-// the same without sums to add to
-__device__ __forceinline__ void mma0(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
-                 : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
-}
 
 // tokens of a request that are attended to
 __device__ __forceinline__ int tokens_of(const PagedParams& p, int len) {
@@ -118,14 +115,13 @@ struct Cfg {
     static constexpr int kSmem = NW * kWarp;
     static_assert(kPart * 4 <= kRing, "the last part lies in the ring");
 };
-struct Yes { static constexpr bool value = true; };
-struct No { static constexpr bool value = false; };
 struct PartMeta { int b, item, flags, rest; };      // flags 1: valid, 2: holds the head's first step, 4: holds its last; rest: steps behind it
 
 template <typename C>
 __global__ void __launch_bounds__(C::NW * 32, 1)
 paged_attn_kernel(const PagedParams p) {
     constexpr int D = C::D, GP = C::GP, TOK = C::TOK, NW = C::NW, NST = C::NST, NR = GP / 8, KS = D / 16, NT = TOK / 8, CH = D / 8, ROWS = 32 / CH;
+    constexpr bool EACH = D == 256;          // a step's sums are added to the others as they come: keeping them elsewhere takes registers that there are not (32 requests of up to 4096 tokens 43 us, 38 this way)
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ long long sm_first[NW * 32], sm_sum[NW];      // sums ahead of every thread's requests in its warp, of the warps
     __shared__ PartMeta sm_meta[NW][2];
@@ -149,7 +145,7 @@ paged_attn_kernel(const PagedParams p) {
     long long off;
     if (lane < 2) sm_meta[warp][lane].flags = 0;
     if (p.B <= 32) {
-        // a lane a request, every warp for itself: one request of 2049 tokens, replayed, 8.4 us; by the sums below 9.0
+        // a lane a request, every warp for itself: one request of 2049 tokens, replayed, 0.6 us less than by the sums below
         const int len = lane < p.B ? tokens_of(p, p.lengths[lane]) : 0, size = size_of(len);
         long long upto = size;
 #pragma unroll
@@ -267,9 +263,33 @@ paged_attn_kernel(const PagedParams p) {
         for (int i = 0; i < NST; ++i) { ask(i); see(); copy_commit(); }
 
         uint32_t qf[KS][2 * NR];
-        float acc[D / 8][4], m[NR], l[NR];
-        bool fresh = true, from_start = false;
+        float acc[D / 8][4], m[NR], l[NR], m_kept[NR];
+        bool fresh = true, from_start = false, kept = false;
         const int g = lane >> 2, c2 = (lane & 3) * 2;
+        float4* const sums = p.kept + (size_t)(cta * NW + warp) * (GP * D / 4) + lane;
+        // with one row a lane the second terms' sums, rows 8 to 15, go to those of the first ones
+        auto one_row = [&]() {
+            if constexpr (NR == 1) {
+#pragma unroll
+                for (int n = 0; n < D / 8; ++n) { acc[n][0] += acc[n][2]; acc[n][1] += acc[n][3]; }
+            }
+        };
+        // float4 i of a lane's sums: two columns of both rows, or of one row in two blocks of columns
+        constexpr int NS = D * NR / 16;
+        auto half = [&](int i, int h) -> float* { return NR == 1 ? acc[2 * i + h] : acc[i] + 2 * h; };
+        auto add_kept = [&]() {
+            if (!kept) return;
+            float f[NR];
+#pragma unroll
+            for (int r = 0; r < NR; ++r) f[r] = m_kept[r] == m[r] ? 1.f : ex2f(m_kept[r] - m[r]);
+#pragma unroll
+            for (int i = 0; i < NS; ++i) {
+                const float4 o = sums[i * 32];
+                float *const a = half(i, 0), *const b = half(i, 1);
+                a[0] += f[0] * o.x; a[1] += f[0] * o.y;
+                b[0] += f[NR - 1] * o.z; b[1] += f[NR - 1] * o.w;
+            }
+        };
 #pragma unroll 1
         for (int step = 0, slot = 0;; ++step) {
             const int4 st = sm_step[warp][step % (2 * NST)];
@@ -291,6 +311,23 @@ paged_attn_kernel(const PagedParams p) {
                     for (int e = 0; e < 4; ++e) acc[n][e] = 0.f;
 #pragma unroll
                 for (int r = 0; r < NR; ++r) { m[r] = -INFINITY; l[r] = 0.f; }
+                kept = false;
+            }
+            if (!EACH && __builtin_expect((step + 1) % kCut == 0, 0)) {
+                one_row();
+                add_kept();
+#pragma unroll
+                for (int i = 0; i < NS; ++i) {
+                    const float *const a = half(i, 0), *const b = half(i, 1);
+                    sums[i * 32] = make_float4(a[0], a[1], b[0], b[1]);
+                }
+#pragma unroll
+                for (int n = 0; n < D / 8; ++n)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) acc[n][e] = 0.f;
+#pragma unroll
+                for (int r = 0; r < NR; ++r) m_kept[r] = m[r];
+                kept = true;
             }
             copy_wait<NST - 1>();
             __syncwarp();
@@ -382,30 +419,35 @@ paged_attn_kernel(const PagedParams p) {
                 for (int n = 0; n < NT; n += 2)
 #pragma unroll
                     for (int j = 0; j < D / 16; j += 2) {
-                        // four independent products between two that add to the same sums, which are those of this step
+                        // four independent products between two that add to the same sums
+                        float sum[4][4];
                         uint32_t b[2][4];
 #pragma unroll
                         for (int i = 0; i < 2; ++i) ldm4t(b[i], base + n * 8 * (D * 2) + (((2 * (j + i) + upper) ^ (lane & 7)) << 4));
-                        float sum[4][4];
-                        auto add = [&](auto first, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3) {
+                        if (EACH) {
 #pragma unroll
-                            for (int i = 0; i < 4; ++i) {
-                                if constexpr (first.value) mma0(sum[i], a0, a1, a2, a3, b[i >> 1][2 * (i & 1)], b[i >> 1][2 * (i & 1) + 1]);
-                                else mma(sum[i], a0, a1, a2, a3, b[i >> 1][2 * (i & 1)], b[i >> 1][2 * (i & 1) + 1]);
-                            }
+                            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                                for (int e = 0; e < 4; ++e) sum[i][e] = 0.f;
+                        }
+                        auto add = [&](uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3) {
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) mma(EACH ? sum[i] : acc[2 * j + i], a0, a1, a2, a3, b[i >> 1][2 * (i & 1)], b[i >> 1][2 * (i & 1) + 1]);
                         };
                         if constexpr (NR == 1) {
-                            add(Yes{}, hi[n][0], mid[n][0], hi[n + 1][0], mid[n + 1][0]);
-                            add(No{}, lo[n][0], 0u, lo[n + 1][0], 0u);
+                            add(hi[n][0], mid[n][0], hi[n + 1][0], mid[n + 1][0]);
+                            add(lo[n][0], 0u, lo[n + 1][0], 0u);
                         } else {
-                            add(Yes{}, hi[n][0], hi[n][1], hi[n + 1][0], hi[n + 1][1]);
-                            add(No{}, mid[n][0], mid[n][1], mid[n + 1][0], mid[n + 1][1]);
-                            add(No{}, lo[n][0], lo[n][1], lo[n + 1][0], lo[n + 1][1]);
+                            add(hi[n][0], hi[n][1], hi[n + 1][0], hi[n + 1][1]);
+                            add(mid[n][0], mid[n][1], mid[n + 1][0], mid[n + 1][1]);
+                            add(lo[n][0], lo[n][1], lo[n + 1][0], lo[n + 1][1]);
                         }
+                        if (EACH) {
 #pragma unroll
-                        for (int i = 0; i < 4; ++i)
+                            for (int i = 0; i < 4; ++i)
 #pragma unroll
-                            for (int e = 0; e < 4; ++e) acc[2 * j + i][e] += sum[i][e];
+                                for (int e = 0; e < 4; ++e) acc[2 * j + i][e] += sum[i][e];
+                        }
                     }
             }
             const bool over = step + 1 == seen, done = (st.z + 1) * TOK >= st.w;
@@ -421,10 +463,8 @@ paged_attn_kernel(const PagedParams p) {
                     l[r] += __shfl_xor_sync(0xFFFFFFFFu, l[r], 1);
                     l[r] += __shfl_xor_sync(0xFFFFFFFFu, l[r], 2);
                 }
-                if constexpr (NR == 1) {
-#pragma unroll
-                    for (int n = 0; n < D / 8; ++n) { acc[n][0] += acc[n][2]; acc[n][1] += acc[n][3]; }
-                }
+                one_row();
+                add_kept();
                 if (done && from_start) {
 #pragma unroll
                     for (int r = 0; r < NR; ++r) {
@@ -616,11 +656,15 @@ int launch_paged(const PagedParams& p, int ctas, cudaStream_t stream) {
 
 }  // namespace
 
-// floats of a CTA's parts: two of the CTA's, one of each warp's
-static long long part_floats(int Hq, int Hkv, int d) { return (long long)(d == 256 ? 4 + 2 : 8 + 2) * (Hq / Hkv > 8 ? 16 : 8) * (d + 4); }
+// warps of a CTA, query heads of a part
+static int warps_of(int d) { return d == 256 ? 4 : 8; }
+static int rows_of(int Hq, int Hkv) { return Hq / Hkv > 8 ? 16 : 8; }
+// floats of a CTA's parts, two of the CTA's and one of each warp's, and of the sums that its warps keep
+static long long part_floats(int Hq, int Hkv, int d) { return (long long)(warps_of(d) + 2) * rows_of(Hq, Hkv) * (d + 4); }
+static long long kept_floats(int Hq, int Hkv, int d) { return d == 256 ? 0 : (long long)warps_of(d) * rows_of(Hq, Hkv) * d; }
 
 long long paged_attn_ws_bytes(int Hq, int Hkv, int head_dim) {
-    return (long long)sms_of_current_device() * (part_floats(Hq, Hkv, head_dim) * (long long)sizeof(float) + (long long)sizeof(int4));
+    return (long long)sms_of_current_device() * ((part_floats(Hq, Hkv, head_dim) + kept_floats(Hq, Hkv, head_dim)) * (long long)sizeof(float) + (long long)sizeof(int4));
 }
 
 int launch_paged_attn(const PagedAttnArgs& a, void* ws, long long ws_bytes, cudaStream_t stream) {
@@ -630,8 +674,9 @@ int launch_paged_attn(const PagedAttnArgs& a, void* ws, long long ws_bytes, cuda
     p.q = (const __nv_bfloat16*)a.q; p.ldq = a.ldq; p.k = (const __nv_bfloat16*)a.k_pages; p.v = (const __nv_bfloat16*)a.v_pages;
     p.page16 = (unsigned)(a.page_stride / 8); p.tok16 = (unsigned)(a.tok_stride / 8);
     p.table = a.table; p.ldt = a.ldt; p.lengths = a.lengths; p.out = (__nv_bfloat16*)a.out; p.ldo = a.ldo; p.bad = a.bad;
-    p.parts = (float*)ws;
-    p.heads = (int4*)((char*)ws + ctas * part_floats(a.Hq, a.Hkv, a.head_dim) * (long long)sizeof(float));
+    p.kept = (float4*)ws;
+    p.parts = (float*)ws + ctas * kept_floats(a.Hq, a.Hkv, a.head_dim);
+    p.heads = (int4*)(p.parts + ctas * part_floats(a.Hq, a.Hkv, a.head_dim));
     p.B = a.B; p.width = a.width; p.page = a.page_size; p.n_pages = a.n_pages; p.Hq = a.Hq; p.Hkv = a.Hkv; p.G = a.Hq / a.Hkv;
     p.blocks = (p.G + 15) / 16; p.items = a.Hkv * p.blocks;
     p.shift = -1;
