@@ -256,7 +256,8 @@ int launch_adjust(const AdjustLogitsArgs& a, cudaStream_t stream) {
     AdjParams p = {a.logits, a.ld, a.out, a.ldo, (const long long*)a.tokens, a.ldk, a.lengths, a.prompt_lengths, a.repetition, a.presence, a.frequency, (const long long*)a.bias_ids, a.bias,
                    a.ldb, a.mask, a.ldm, a.repetition_all, a.presence_all, a.frequency_all, a.V, a.max_tokens, a.n_bias, 0};
     // Segments of a row: as few as shared memory allows, since every one reads all of the row's tokens, unless SMs would have nothing to do; then as many as the last round of CTAs has room for
-    // (64 rows of 151936 with 4096 tokens and 100 biases: 4 of 38912 in one round 15.5 us; with counts of 32 bits 9 of 17408 in two rounds 18.5, 10 of 16384 in three 20.5).
+    // (64 rows of 151936 with 4096 tokens and 100 biases: 4 of 38912 in one round 15.8 us; with counts of 32 bits 9 of 17408 in two rounds 18.5, 10 of 16384 in three 20.5).
+    // Counted as two CTAs of 512 threads an SM; histories near 8192 tokens beside thousands of biases take the shared memory of one, and a second round.
     const long long slots = 1024ll / kAdjThreads * sms_of_current_device();
     long long n = ((long long)a.V + kLargest - 1) / kLargest;
     const long long rounds = (a.rows * n + slots - 1) / slots, most = ((long long)a.V + 2047) / 2048;
@@ -279,7 +280,7 @@ int launch_adjust(const AdjustLogitsArgs& a, cudaStream_t stream) {
 }  // namespace
 
 int launch_adjust_logits(int dtype, const AdjustLogitsArgs& a, cudaStream_t stream) {
-    // Long histories, which every CTA of a row reads, are read by fewer CTAs of twice the threads (8 rows of 151936 with 30000 tokens 13.3 -> 10.8 us; 64 rows with 4096 tokens 15.5, 20.9 that way).
+    // Long histories, which every CTA of a row reads, are read by fewer CTAs of twice the threads (8 rows of 151936 with 30000 tokens 13.3 -> 11.0 us; 64 rows with 4096 tokens 15.8, 20.9 that way).
     if (a.lengths && a.max_tokens > kAdjShort) return dtype == 1 ? launch_adjust<float, 1024>(a, stream) : launch_adjust<__nv_bfloat16, 1024>(a, stream);
     return dtype == 1 ? launch_adjust<float, 512>(a, stream) : launch_adjust<__nv_bfloat16, 512>(a, stream);
 }

@@ -100,7 +100,7 @@ page_plan_kernel(const PagePlanArgs a) {
     }
     __syncthreads();
 
-    // rows, kPlanRowsAtOnce of a thread side by side: a search is a chain of shared-memory reads. Bound by issue on the cluster's few SMs (32768 rows of 1000 requests 8.6 us, 9.9 with a branch in the search).
+    // rows, kPlanRowsAtOnce of a thread side by side: a search is a chain of shared-memory reads. Bound by issue on the cluster's few SMs (32768 rows of 1000 requests 8.2 us, 9.9 with a branch in the search).
     for (int r0 = cta * kPlanThreads + tid; r0 < a.max_rows; r0 += ctas * kPlanThreads * kPlanRowsAtOnce) {
         int lo[kPlanRowsAtOnce], hi[kPlanRowsAtOnce];
 #pragma unroll

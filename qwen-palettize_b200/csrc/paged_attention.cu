@@ -11,13 +11,14 @@
 //     Weights are three bf16 terms of the fp32 value, all 24 bits of it (two terms, 16 bits, differed from the sums in fp32 in the last bit of 0.2 % of the results). With up to 8 query heads
 //     the second terms are rows 8 to 15 of the same product and cost nothing, the third are a product of their own: 256 short requests 39.9 -> 41.0 us, long ones within 1 %.
 //     The accumulators of the products cut what falls below their last bit instead of rounding it: after n steps about n 2^-24 of a sum is gone (32 requests of 131072 tokens, 3500 steps a warp:
-//     2.1 % of the results off in their last bit). So a warp's sums of 64 steps are added to earlier ones in fp32, rounded to nearest, which a lane keeps for itself in the workspace (0.02 %;
-//     2 x 131072 tokens 165.6 -> 168.6 us; a step's sums added by themselves 166.5, but 182 where 172 is reached with the clocks of sustained load); with heads of 256, those of a step.
+//     2.1 % of the results off in their last bit). So a warp's sums of 32 steps are added to earlier ones in fp32, rounded to nearest, which a lane keeps for itself in the workspace: then as many
+//     results are off as with sums in fp32 throughout (64 requests of up to 4096 tokens 0.06 %, 2 x 131072 0.07 %). Replayed, without / 64 / 32 / 16 / 8 steps: 99 / 99.6 / 101.3 / 103.8 / 105 us
+//     and 166 / 169 / 172 / 176 / 178; a step's sums added by themselves 100 and 167, but 182 where 32 steps take 176 and none 169, with the clocks of sustained load. With heads of 256, those of a step.
 //     The reference of the exponentials moves when a row's maximum has grown by more than 2^8.
 //     A head that a warp finishes alone goes to `out`; parts meet in shared memory at the end, parts that cross CTAs go to the workspace, two per CTA at most.
 //   paged_join_kernel  one block per CTA of the first kernel and query head of a group joins the parts of the head that began there and went on; most have nothing to do.
 //
-// Measured, replayed (query / key heads 32 / 8 of 128, pages of 16 or 64): 2 x 131072 tokens 166 to 169 us for 1.07 GB, 6.4 TB/s; 64 requests of up to 4096 tokens 99 us for 0.58 GB, 5.8 TB/s; 256 requests
+// Measured, replayed (query / key heads 32 / 8 of 128, pages of 16 or 64): 2 x 131072 tokens 169 to 172 us for 1.07 GB, 6.3 TB/s; 64 requests of up to 4096 tokens 101 us for 0.58 GB, 5.7 TB/s; 256 requests
 // of up to 300 tokens, 16 / 16 heads of 64, 39 us for 0.16 GB; one request of 2049 tokens 8.6 us, a chain of latencies: lengths, pages, keys, two meetings, a second launch. Heads 8 / 2 of 256,
 // 32 requests of up to 4096 tokens, 38 us for 0.12 GB; 32 / 2 of 128, 64 such requests, 44 us for 0.14 GB.
 //   What is in flight matters (before the third term and the kept sums): three steps a warp (196 KB of copies per SM) 187 and 110 us for the first two, since SMs then starve one another (their times
@@ -28,7 +29,7 @@ namespace plz {
 namespace {
 
 constexpr int kSwitch = 2;               // steps that the change to another head counts on the line (0: 256 short requests 45 us; 1, 2: 37; 4: 39)
-constexpr int kCut = 64;                 // steps after which a warp's sums are kept elsewhere and begun anew
+constexpr int kCut = 32;                 // steps after which a warp's sums are kept elsewhere and begun anew
 constexpr float kGrow = 8.f;             // exponents (base 2) that a maximum may grow before the reference moves
 constexpr float kLog2e = 1.4426950408889634f;
 
