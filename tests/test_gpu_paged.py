@@ -309,6 +309,36 @@ def test_long_sums_do_not_drift(hq, hk, d):
     assert float((got.double() != want.bfloat16().double()).double().mean()) <= 2 * e * 2 ** 8
 
 
+@pytest.mark.parametrize("hq,hk,d", [(8, 1, 64), (3, 1, 128), (12, 1, 128), (2, 1, 256)])
+@pytest.mark.parametrize("shape", ["rising", "falling", "saw", "back and forth"])
+def test_references_that_move_over_many_steps(hq, hk, d, shape):
+    """Scores between -40 and 0 that go up or down again and again within a warp's 150 steps, so that sums of earlier steps count for nothing, for everything or in part. Columns are the parts of the period.
+    A weight is off by 2 ((d + 4) 2^-23 40 + 2^-21), a sum of positive products by 2^-23 for each of a warp's 16 * 150 tokens and 2400 parts, and bf16 by 2^-8, all of itself."""
+    import plz_ops as ops
+    tok, warps = (32 if d == 64 else 16), (4 if d == 256 else 8) * torch.cuda.get_device_properties(0).multi_processor_count
+    page, period = 64, 100 * tok + 37
+    n = 150 * warps * tok // page * page + 5
+    pos = torch.arange(n, device="cuda")
+    x = (pos % period).double() / period
+    s = {"rising": 40 * (pos.double() / n - 1), "falling": -40 * pos.double() / n, "saw": -40 * x, "back and forth": -80 * (x - 0.5).abs()}[shape].bfloat16()
+    part = pos * d // n if shape in ("rising", "falling") else pos % period * d // period
+    pages = -(-n // page)
+    g = torch.Generator(device="cuda").manual_seed(d)
+    table = torch.randperm(pages, generator=g, device="cuda").to(I32)[None]
+    at = table[0, pos // page].long() * page + pos % page
+    kp, vp = (torch.zeros(pages, page, d, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    kp.view(-1, d)[at, 0] = s
+    vp.view(-1, d)[at, part] = 1.0
+    q = torch.zeros(1, hq, d, dtype=torch.bfloat16, device="cuda")
+    q[0, :, 0] = torch.tensor([1.0, 0.5, 0.25], device="cuda").repeat(4)[:hq]
+    got = ops.attention_decode_paged(q.view(1, -1), kp, vp, table, _dev([n]), hq, hk, d, scale=1.0).view(hq, d).double()
+    check_status()
+    w = (s.double() * q[0, :, :1].double()).exp()
+    want = torch.zeros(hq, d, dtype=torch.float64, device="cuda").index_add_(1, part, w / w.sum(1, keepdim=True))
+    rel = 2.0 ** -8 * (1 + 2.0 ** -8) + 2 * (2 * ((d + 4) * 2.0 ** -23 * 40 + 2.0 ** -21) + (16 * 150 + 2400) * 2.0 ** -23)
+    assert ((got - want).abs() <= rel * want + 2.0 ** -126).all(), float(((got - want).abs() / (rel * want)).nan_to_num().max())
+
+
 @pytest.mark.parametrize("B", [2, 31, 32, 33, 64])
 @pytest.mark.parametrize("hq,hk,d", [(8, 2, 128), (20, 1, 64), (4, 4, 256)])
 @pytest.mark.parametrize("holes", ["none", "ends", "inside", "most"])
